@@ -49,6 +49,11 @@ def _signatures():
             c_int,
             [c_void_p] * 6 + [c_int64] * 12 + [c_int, c_int, c_float, c_int, c_void_p, c_int64, c_int, c_void_p],
         ),
+        "b200ait_gemm_rcr_i8": (c_int, [c_void_p] * 8 + [c_int64] * 7 + [c_int] * 3 + [c_void_p]),
+        "b200ait_quantize_rows": (c_int, [c_void_p] * 3 + [c_int64] * 4 + [c_int] * 3 + [c_void_p]),
+        "b200ait_residual_norm": (
+            c_int, [c_void_p] * 10 + [c_int64] * 6 + [c_int, c_int, c_float, c_float, c_int, c_void_p],
+        ),
         "b200ait_bmm_permute0213": (
             c_int, [c_void_p] * 3 + [c_int64] * 7 + [c_int, c_int, c_float, c_int, c_void_p],
         ),

@@ -23,7 +23,7 @@
 #include <mutex>
 #include <vector>
 
-#include "gemm_kernel.cuh"
+#include "gemm_swapab.cuh"
 
 namespace b200ait {
 
@@ -80,28 +80,6 @@ __global__ void __launch_bounds__(256) gemm_splitk_reduce_kernel(const GemmParam
   epilogue_chunk32<BF16>(p, v, b, row, col0, true);
 }
 
-// The fused epilogue on one fp32 accumulator: alpha, bias, activation, residual(s), activation, one rounding.
-template <bool BF16>
-__device__ __forceinline__ void epilogue_scalar_store(const GemmParams& p, float acc, int b, int row, int col) {
-  using E = Elem16<BF16>;
-  using T = typename E::T;
-  const int u1 = epi_u1(p.epilogue), b1 = epi_b1(p.epilogue), b2 = epi_b2(p.epilogue), u2 = epi_u2(p.epilogue);
-  float v = acc * p.alpha;
-  if (p.bias) v += E::to_float(static_cast<const T*>(p.bias)[col]);
-  v = apply_unary(u1, v);
-  const long long di = static_cast<long long>(b) * p.d_bs + static_cast<long long>(row) * p.ldd + col;
-  if (b1 != kBinaryNone) {
-    const float f = E::to_float(static_cast<const T*>(p.d0)[di]);
-    v = (b1 == kBinaryAdd) ? v + f : v * f;
-  }
-  if (b2 != kBinaryNone) {
-    const float f = E::to_float(static_cast<const T*>(p.d1)[di]);
-    v = (b2 == kBinaryAdd) ? v + f : v * f;
-  }
-  v = apply_unary(u2, v);
-  static_cast<T*>(p.out)[batch_offset(p, b) + row_offset(p, row) + col_offset(p, col)] = E::from_float(v);
-}
-
 // ------------------------------------------------------------------------------------------------
 // CUDA-core kernel for shapes TMA cannot address. 32x32 output tile per block, K staged in smem.
 template <bool BF16>
@@ -140,6 +118,42 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(const void* a_, const vo
   for (int i = 0; i < 4; ++i) {
     const int row = row0 + ty + i * 8;
     if (row < p.M) epilogue_scalar_store<BF16>(p, acc[i], b, row, col);
+  }
+}
+
+// The same for 8-bit integers whose rows do not start on 16 bytes: 64 elements of K at a time, staged byte by byte as
+// words of four, four products per instruction.
+template <bool BF16>
+__global__ void __launch_bounds__(256) gemm_simt_i8_kernel(const int8_t* a, const int8_t* w, const GemmParams p) {
+  constexpr int kWords = 16;
+  __shared__ int sa[32][kWords + 1];
+  __shared__ int sb[32][kWords + 1];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;  // 32 x 8
+  const int row0 = blockIdx.y * 32, col0 = blockIdx.x * 32;
+  int acc[4] = {0, 0, 0, 0};
+  for (int k0 = 0; k0 < p.K; k0 += 4 * kWords) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = threadIdx.x + 256 * i, r = e >> 6, kk = e & 63, k = k0 + kk;
+      reinterpret_cast<int8_t*>(sa[r])[kk] = row0 + r < p.M && k < p.K ? a[static_cast<long long>(row0 + r) * p.lda + k] : int8_t{0};
+      reinterpret_cast<int8_t*>(sb[r])[kk] = col0 + r < p.N && k < p.K ? w[static_cast<long long>(col0 + r) * p.ldb + k] : int8_t{0};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kWords; ++q) {
+      const int bv = sb[tx][q];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = __dp4a(sa[ty + i * 8][q], bv, acc[i]);
+    }
+    __syncthreads();
+  }
+  const int col = col0 + tx;
+  if (col >= p.N) return;
+  const float cs = p.col_scale[col];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = row0 + ty + i * 8;
+    if (row < p.M) epilogue_scalar_store_i8<BF16>(p, __int2float_rn(acc[i]) * cs, row, col);
   }
 }
 
@@ -286,518 +300,13 @@ __global__ void __launch_bounds__(kRowDotShortThreads, 1) gemm_rowdot_short_kern
 }
 
 // ------------------------------------------------------------------------------------------------
-// Weight-streaming tensor-core kernel with the operands swapped: Y^T = W X^T.
-// The run time of a GEMM with few rows of X is the time to read W once. Here the rows of W sit on the 128 MMA rows
-// and the rows of X are the MMA's N (MX = 16 .. 256), so a CTA consumes 16 KB of weights per four MMAs, and W is
-// partitioned so that every byte is read by exactly one CTA per group of MX rows of X: a cluster of R = 2, 4 or 8 CTAs
-// owns a slab of 128 weight rows, rank r streams share r of K through a TMA ring, and the ranks hand each other
-// their 128 x MX fp32 partial sums through the cluster's shared-memory window (a reduce-scatter: every rank finishes
-// MX / R rows of X). No global workspace, no second pass (the 128 x 256 tiles + split-K + reduce kernel this
-// replaces ran at 0.54 of the copy rate for M <= 32). More than 256 rows of X are taken in groups of 256.
-//   warp 0: TMA producer   warp 1: MMA issuer   warps 2-5: epilogue (TMEM lane = weight row = output column)
-constexpr int kSwapThreads = 192;
-constexpr int kSwapMaxM = 256;
-template <int MX, int R, int H>
-struct SwapCfg {
-  static_assert(R == 1 || R == 2 || R == 4 || R == 8, "cluster size");
-  static constexpr int kPart = MX / R;              // rows of X each rank finishes ...
-  static constexpr int kSub = kPart / H;            // ... in H passes of kSub rows (what bounds the exchange buffers)
-  static_assert(H >= 1 && kSub * H == kPart && kSub >= 8, "a rank finishes at least 8 rows per pass");
-  static constexpr int kWBytes = 128 * kBK * 2;     // 16 KB: 128 weight rows x 64 k
-  static constexpr int kXBytes = MX * kBK * 2;      // MX rows of X x 64 k
-  static constexpr int kStageBytes = kWBytes + kXBytes;
-  static constexpr int kSlotBytes = 128 * kSub * 4;                // [kSub rows of X][128 weight rows] fp32
-  static constexpr int kPartialBytes = (R - 1) * kSlotBytes;       // one slot per peer: its sums for this rank's rows
-  static constexpr int kTileBytes = kSlotBytes;                    // the finished tile, [kSub][128]
-  static constexpr int kFit = (227 * 1024 - 256 - kPartialBytes - kTileBytes) / kStageBytes;
-  static constexpr int kStages = kFit < 8 ? kFit : 8;  // 144 to 192 KB in flight
-  static constexpr int kAccCols = MX < 32 ? 32 : MX;  // TMEM columns of one accumulator
-  static constexpr int kTmemCols = 2 * kAccCols;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kPartialBytes + kTileBytes + 256;
-  static_assert(kStages >= 3 && kSmemBytes <= 227 * 1024, "swapped-operand kernel: shared memory");
-};
-
-template <int N>
-__device__ __forceinline__ void tmem_ld_chunk(uint32_t taddr, uint32_t (&r)[N]) {
-  static_assert(N == 8 || N == 16 || N == 32, "TMEM load width");
-  if constexpr (N == 8) {
-    tmem_ld_32x32b_x8(taddr, r);
-  } else if constexpr (N == 16) {
-    tmem_ld_32x32b_x16(taddr, r);
-  } else {
-    tmem_ld_32x32b_x32(taddr, r);
-  }
-}
-
-template <bool BF16, int MX, int R, int H>
-__global__ void __launch_bounds__(kSwapThreads, 1)
-gemm_swapab_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
-                   const GemmParams p, const int num_slabs, const int num_groups) {
-  using Cfg = SwapCfg<MX, R, H>;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  const bool misaligned = (smem_u32(smem) & 1023u) != 0u;
-  if (misaligned && threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kDevBadSmemAlignment);
-  float* partial = reinterpret_cast<float*>(smem + Cfg::kStages * Cfg::kStageBytes);  // [R - 1][kSub / 4][128][4], a slot per peer
-  float* tile = reinterpret_cast<float*>(smem + Cfg::kStages * Cfg::kStageBytes + Cfg::kPartialBytes);  // [kSub][128]
-  uint64_t* full_bar =
-      reinterpret_cast<uint64_t*>(smem + Cfg::kStages * Cfg::kStageBytes + Cfg::kPartialBytes + Cfg::kTileBytes);
-  uint64_t* empty_bar = full_bar + Cfg::kStages;
-  uint64_t* acc_full = empty_bar + Cfg::kStages;   // [2]
-  uint64_t* acc_empty = acc_full + 2;             // [2]
-  uint64_t* partial_ready = acc_empty + 2;        // every peer's partial sums are in `partial` (counts their bytes)
-  uint64_t* partial_taken = partial_ready + 1;    // [2] every peer has read the sums it was sent (even / odd passes)
-  uint64_t* drain_bar = partial_taken + 2;
-  uint64_t* tile_summed = drain_bar + 1;          // every thread has put its sums into `tile`
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tile_summed + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 * Cfg::kStages + 9) * 8 + 8 <= 256, "barrier area too small");
-
-  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_ctarank());
-  const int walker = blockIdx.x / R, num_walkers = gridDim.x / R;
-  // a unit of work: one slab of 128 weight rows against one group of MX rows of X (consecutive units share the slab,
-  // so the clusters that run them side by side fetch its weights from HBM once)
-  const int my_units = misaligned ? 0 : num_slabs * num_groups;
-  // this rank's share of the k-blocks (the host sends no problem with fewer k-blocks than ranks)
-  const int kb_total = (p.K + kBK - 1) / kBK;
-  // split evenly, so that no rank is left without a k-block (its accumulator would never be written)
-  const int kb0 = rank * kb_total / R, kb1 = (rank + 1) * kb_total / R;
-
-  // Set-up, kept short because a small problem's whole run is a few microseconds: the lanes of warp 0 initialise one
-  // barrier each while warp 1 allocates tensor memory, and the opening cluster barrier is arrived at without a release
-  // (the initialisations are published by fence.mbarrier_init; a releasing arrive alone was measured at 0.5 us). Only the
-  // epilogue warps touch the peers, so only they wait for the cluster here: the producer goes on to its loads as soon as its
-  // barriers stand, the MMA issuer once tensor memory is there too, and both wait for the cluster after their work.
-  constexpr int kSetupBar = 1;
-  if (warp == 0) {
-    // barriers in the order they lie in shared memory: full[kStages], empty[kStages], acc_full[2], acc_empty[2],
-    // partial_ready, partial_taken[2], drain_bar, tile_summed
-    constexpr int kBars = 2 * Cfg::kStages + 9;
-    for (int i = lane; i < kBars; i += 32) {
-      const int j = i - 2 * Cfg::kStages;  // index among the barriers after the ring's
-      // every epilogue thread arrives at acc_empty and tile_summed, every peer's at partial_taken, one thread elsewhere
-      const uint32_t count = (j == 2 || j == 3 || j == 8) ? 128u : (j == 5 || j == 6) ? 128u * (R > 1 ? R - 1 : 1) : 1u;
-      mbar_init(&full_bar[i], count);
-    }
-    if (lane == 0) *abort_flag = 0;
-    fence_mbar_init();
-    fence_proxy_async_smem();  // the loads below credit barriers that other lanes have initialised
-    __syncwarp();
-  } else if (warp == 1) {
-    tmem_alloc(tmem_slot, Cfg::kTmemCols);  // two accumulators
-    grid_release();
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  cluster_arrive_relaxed();
-  if (warp == 0) {
-    named_bar_arrive(kSetupBar, kSwapThreads);
-  } else {
-    named_bar_sync(kSetupBar, kSwapThreads);
-    if (warp != 1) cluster_wait();  // the peers' barriers are initialised before anything signals them
-  }
-  tc_fence_after();
-  grid_wait();
-  bool epi_arrived = false;  // this thread has arrived at the closing cluster barrier
-
-  if (warp == 0) {
-    // TMA producer. Every CTA reads the same rows of X: walking the k-blocks from a different starting point in every
-    // cluster keeps the CTAs from asking L2 for the same lines of X at the same moment.
-    const uint32_t lead = elect_one();
-    const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(full_bar);
-    const int nkb = kb1 - kb0;
-    int stage = 0;
-    uint32_t phase = 0;
-    bool first = true;  // the first pass over the ring: every stage is free
-    bool ok = true;
-    for (int unit = walker; ok && unit < my_units; unit += num_walkers) {
-      const int slab = unit / num_groups, grp = unit - slab * num_groups;
-      // (by slab, not by unit: every group of X rows adds its k-blocks up in the same order, so a row's result does not
-      // depend on the group it falls into)
-      const int rot = nkb > 0 ? static_cast<int>((static_cast<unsigned>(slab) * 11u) % static_cast<unsigned>(nkb)) : 0;
-      for (int i = 0; i < nkb; ++i) {
-        const int kb = kb0 + (i + rot >= nkb ? i + rot - nkb : i + rot);
-        if (!first) ok = mbar_wait_warp(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, kDevWaitEmptyTimeout);
-        if (!ok) break;
-        const uint32_t sw = smem0 + static_cast<uint32_t>(stage) * Cfg::kStageBytes, bar = full0 + static_cast<uint32_t>(stage) * 8u;
-        mbar_arrive_expect_tx_warp(&full_bar[stage], Cfg::kStageBytes, lead);
-        tma_load_3d_warp(sw, &tma_w, bar, kb * kBK, slab * 128, 0, lead);
-        tma_load_3d_warp(sw + Cfg::kWBytes, &tma_x, bar, kb * kBK, grp * MX, 0, lead);
-        if (++stage == Cfg::kStages) {
-          stage = 0;
-          phase ^= 1u;
-          first = false;
-        }
-      }
-    }
-    if (!ok) {
-      const uint64_t t0 = globaltimer_ns();
-      while (globaltimer_ns() - t0 < 200000ull) {
-      }
-    }
-    __syncwarp();
-    cluster_wait();
-  } else if (warp == 1) {
-    constexpr uint32_t idesc = umma_idesc_f16(128, MX, BF16, false, false);
-    const uint32_t tmem_base = *tmem_slot;
-    const uint32_t lead = elect_one();
-    int stage = 0;
-    uint32_t phase = 0;
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    bool ok = true;
-    for (int unit = walker; ok && unit < my_units; unit += num_walkers) {
-      ok = mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1u, abort_flag, p.status, kDevWaitAccEmptyTimeout);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * Cfg::kAccCols);
-      for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mbar_wait_warp(&full_bar[stage], phase, abort_flag, p.status, kDevWaitFullTimeout);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t w_addr = smem_u32(smem + stage * Cfg::kStageBytes);
-        const uint32_t w_lo = umma_smem_desc_sw128_lo(w_addr, 16), x_lo = umma_smem_desc_sw128_lo(w_addr + Cfg::kWBytes, 16);
-#pragma unroll
-        for (int k = 0; k < kBK / 16; ++k)
-          umma_f16_ss_warp(d_tmem, w_lo + k * (32 >> 4), x_lo + k * (32 >> 4), idesc, (kb > kb0 || k != 0) ? 1u : 0u, lead);
-        umma_commit_warp(&empty_bar[stage], lead);
-        if (++stage == Cfg::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-      if (!ok) break;
-      umma_commit_warp(&acc_full[acc], lead);
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
-    }
-    if (!ok) {
-      umma_commit_warp(drain_bar, lead);
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(drain_bar, 0) && globaltimer_ns() - t0 < 1000000ull) {
-      }
-    }
-    __syncwarp();
-    cluster_wait();
-  } else {
-    const uint32_t tmem_base = *tmem_slot;
-    // The MX rows of X are cut into H x R blocks of kSub rows; in pass h rank r finishes block h * R + r: it keeps
-    // that block of its own sums and sends each peer q the block h * R + q (slot "sender" of q's `partial`, four rows
-    // of X per 16-byte store: a warp's store covers 512 consecutive bytes). The stores are asynchronous and credit their bytes to the receiver's
-    // `partial_ready`: nobody waits for a store to land except the thread that needs the data. Then the rank adds
-    // what its peers sent into `tile` and writes its rows out. (H > 1 only bounds the buffers: 256 rows of X would
-    // otherwise need 128 KB of them.)
-    constexpr int kSub = Cfg::kSub;
-    constexpr int kChunk = kSub < 32 ? kSub : 32;  // TMEM columns per load
-    const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;  // weight row inside the slab == TMEM lane
-    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const int et = static_cast<int>(threadIdx.x) - 64;  // 0..127 over the four epilogue warps
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    // Passes done so far: `tile_summed` changes phase once per pass. The peers' "taken" signals of pass s go to
-    // partial_taken[s & 1]: a rank that has no rows in a pass runs through it without waiting for anybody's sums, so
-    // its signals of pass s + 1 can be complete before a slow thread here has looked at those of pass s. With one
-    // barrier that thread would then wait on a parity that has come round again; with two, a barrier is reused only
-    // for pass s + 2, which no peer can finish before every thread here has signalled pass s + 1.
-    int seq = 0;
-    uint32_t ready_phase = 0;  // `partial_ready` only changes phase in the passes in which this rank has rows
-    bool ok = true;
-    for (int unit = walker; ok && unit < my_units; unit += num_walkers) {
-      const bool last_slab = unit + num_walkers >= my_units;
-      const int slab = unit / num_groups;
-      const int row_base = (unit - slab * num_groups) * MX;  // first row of X of this unit's group
-      const int m_here = p.M - row_base < MX ? p.M - row_base : MX;
-      // The tile goes out row by row: a thread takes 8 consecutive columns (one 16-byte store), 16 threads one
-      // row of the slab. A thread keeps the same columns for every row, so it fetches their bias once, early.
-      const int col0 = slab * 128 + (et & 15) * 8;
-      const bool vec = p.vec_ok && col0 + 8 <= p.N;
-      float bias_v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (vec && p.bias != nullptr)
-        unpack8<BF16>(*reinterpret_cast<const uint4*>(static_cast<const typename Elem16<BF16>::T*>(p.bias) + col0), bias_v);
-      ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, kDevWaitAccFullTimeout);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t t_addr = tmem_base + lane_addr + static_cast<uint32_t>(acc * Cfg::kAccCols);
-#pragma unroll 1
-      for (int pass = 0; ok && pass < H; ++pass, ++seq) {
-      const bool last = last_slab && pass == H - 1;
-      const int my_row0 = (pass * R + rank) * kSub;
-      const int my_rows = m_here - my_row0 < 0 ? 0 : (m_here - my_row0 < kSub ? m_here - my_row0 : kSub);
-      const int out_row0 = row_base + my_row0;  // where this rank's block starts in the output
-      // what the peers will send for this pass (a rank with no valid row of X is sent nothing and waits for nothing)
-      if (R > 1 && et == 0 && my_rows > 0) mbar_arrive_expect_tx(partial_ready, (R - 1) * Cfg::kSlotBytes);
-      // the peers must have read what this CTA sent for the previous pass before it is overwritten
-      if (R > 1 && seq > 0)
-        ok = mbar_wait_cluster(&partial_taken[(seq - 1) & 1], ((seq - 1) >> 1) & 1, abort_flag, p.status,
-                               kDevWaitOtherTimeout);
-#pragma unroll
-      for (int q = 0; q < R; ++q) {
-        const int q_row0 = (pass * R + q) * kSub;
-        if (q == rank || m_here <= q_row0) continue;
-        const int slot = rank < q ? rank : rank - 1;  // where this rank's sums go in rank q's buffer
-        const uint32_t dst = mapa_shared(smem_u32(partial), static_cast<uint32_t>(q)) +
-                             static_cast<uint32_t>((slot * kSub * 128 + row * 4) * 4);
-        const uint32_t dst_bar = mapa_shared(smem_u32(partial_ready), static_cast<uint32_t>(q));
-#pragma unroll
-        for (int c = 0; c < kSub / kChunk; ++c) {
-          uint32_t v[kChunk];
-          tmem_ld_chunk<kChunk>(t_addr + static_cast<uint32_t>(q_row0 + c * kChunk), v);
-          tmem_ld_wait();
-          if (ok) {
-#pragma unroll
-            for (int j = 0; j < kChunk; j += 4)
-              st_async_cluster_v4(dst + static_cast<uint32_t>((c * kChunk + j) * 128 * 4), v[j], v[j + 1], v[j + 2], v[j + 3],
-                                  dst_bar);
-          }
-        }
-      }
-      // After its last send a thread touches no peer again: the cluster-wide barrier that keeps every CTA alive
-      // until then is arrived at here and waited for at the very end, when it has long completed.
-      if (last) {
-        cluster_arrive_relaxed();
-        epi_arrived = true;
-      }
-      if (ok && my_rows > 0) {
-        if constexpr (R > 1) {
-          ok = mbar_wait_cluster(partial_ready, ready_phase, abort_flag, p.status, kDevWaitOtherTimeout);
-          ready_phase ^= 1u;
-        }
-#pragma unroll
-        for (int c = 0; c < kSub / kChunk; ++c) {
-          uint32_t v[kChunk];
-          tmem_ld_chunk<kChunk>(t_addr + static_cast<uint32_t>(my_row0 + c * kChunk), v);
-          tmem_ld_wait();
-          if (ok) {
-            // The K shares are added in the order of their ranks whichever rank does the adding, so a row's result
-            // does not depend on which rank finishes it (= on its position in X). All loads of the chunk come before
-            // its first store: the compiler may not move a load of `partial` over a store to `tile` by itself.
-            float sum[kChunk];
-#pragma unroll
-            for (int j = 0; j < kChunk; j += 4) {
-#pragma unroll
-              for (int q = 0; q < R; ++q) {
-                const int slot = q < rank ? q : q - 1;  // where rank q's sums sit in this rank's buffer
-                const float4 term =
-                    q == rank ? make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]),
-                                            __uint_as_float(v[j + 3]))
-                              : *reinterpret_cast<const float4*>(partial + ((slot * kSub + c * kChunk + j) * 128 + row * 4));
-                sum[j] = q == 0 ? term.x : sum[j] + term.x;
-                sum[j + 1] = q == 0 ? term.y : sum[j + 1] + term.y;
-                sum[j + 2] = q == 0 ? term.z : sum[j + 2] + term.z;
-                sum[j + 3] = q == 0 ? term.w : sum[j + 3] + term.w;
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) tile[(c * kChunk + j) * 128 + row] = sum[j];
-          }
-        }
-      }
-      if (pass == H - 1) {  // the accumulator has been read for the last time
-        tc_fence_before();
-        mbar_arrive(&acc_empty[acc]);
-      }
-      if (ok) {
-        mbar_arrive(tile_summed);
-        ok = mbar_wait(tile_summed, seq & 1, abort_flag, p.status, kDevWaitOtherTimeout);
-      }
-      if (ok) {
-        const int code = p.epilogue;
-        // bias + one activation [+ one added residual [+ relu]] into a row-major output: the short store loop
-        const bool add_d0 = epi_b1(code) == kBinaryAdd;
-        const bool simple = vec && (epi_b1(code) == kBinaryNone || add_d0) && epi_b2(code) == kBinaryNone &&
-                            (epi_u2(code) == kUnaryIdentity || (add_d0 && epi_u2(code) == kUnaryRelu)) &&
-                            p.store_mode == 0;
-        // An activation that is more than a max runs first, in place on this thread's own elements of the tile, a row
-        // per trip of a rolled loop, so that the store loops below carry no activation code but relu. (This code runs
-        // once or twice per launch, from a cold instruction cache: with the activations dispatched inside the 32-wide
-        // store loop, 3072 x 768 at M = 128 with tanh took 4.7 us longer than with bias alone, 8192 x 8192 9.2 us.)
-        const bool pre = vec && epi_u1(code) != kUnaryIdentity && epi_u1(code) != kUnaryRelu;
-        if (pre) {
-          const int u1 = epi_u1(code);
-#pragma unroll 1
-          for (int j = et >> 4; j < my_rows; j += 8) {
-            float* src = tile + j * 128 + (et & 15) * 8;
-            const float4 a0 = *reinterpret_cast<const float4*>(src), a1 = *reinterpret_cast<const float4*>(src + 4);
-            float w[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = w[e] * p.alpha + bias_v[e];
-            apply_unary_vec(u1, w);
-            *reinterpret_cast<float4*>(src) = make_float4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<float4*>(src + 4) = make_float4(w[4], w[5], w[6], w[7]);
-          }
-        }
-        if (simple) {
-          // four rows (j, j + 8, j + 16, j + 24) per trip, all of a trip's shared-memory loads first; no per-row
-          // dispatch on the epilogue code
-          using T = typename Elem16<BF16>::T;
-          const bool relu = epi_u1(code) == kUnaryRelu, relu_after = epi_u2(code) == kUnaryRelu;
-          T* out0 = static_cast<T*>(p.out) + col0;
-          const T* res0 = static_cast<const T*>(p.d0) + col0;
-          for (int j = et >> 4; j < my_rows; j += 32) {
-            float o[4][8];
-            uint4 r0[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const int jj = j + 8 * t < my_rows ? j + 8 * t : j;
-              if (add_d0) r0[t] = *reinterpret_cast<const uint4*>(res0 + static_cast<long long>(out_row0 + jj) * p.ldd);
-              const float* src = tile + jj * 128 + (et & 15) * 8;
-              const float4 a0 = *reinterpret_cast<const float4*>(src), a1 = *reinterpret_cast<const float4*>(src + 4);
-              o[t][0] = a0.x, o[t][1] = a0.y, o[t][2] = a0.z, o[t][3] = a0.w;
-              o[t][4] = a1.x, o[t][5] = a1.y, o[t][6] = a1.z, o[t][7] = a1.w;
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              if (j + 8 * t < my_rows) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const float y = pre ? o[t][e] : o[t][e] * p.alpha + bias_v[e];
-                  o[t][e] = relu ? fmaxf(y, 0.f) : y;  // identity keeps a NaN a NaN
-                }
-                if (add_d0) {
-                  float f[8];
-                  unpack8<BF16>(r0[t], f);
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) o[t][e] = relu_after ? fmaxf(o[t][e] + f[e], 0.f) : o[t][e] + f[e];
-                }
-                *reinterpret_cast<uint4*>(out0 + static_cast<long long>(out_row0 + j + 8 * t) * p.ldc) = pack8<BF16>(o[t]);
-              }
-            }
-          }
-        }
-        if (!simple && vec) {
-          // Any epilogue: four rows per trip again. A trip's shared-memory loads and residual loads all go out
-          // before the first is used, and each activation is dispatched once per trip, over the 32 values.
-          using T = typename Elem16<BF16>::T;
-          const int u1 = epi_u1(code), b1 = epi_b1(code), b2 = epi_b2(code), u2 = epi_u2(code);
-          T* out0 = static_cast<T*>(p.out) + col_offset(p, col0);
-          for (int j = et >> 4; j < my_rows; j += 32) {
-            float o[32];
-            uint4 r0[4], r1[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const int jj = j + 8 * t < my_rows ? j + 8 * t : j;
-              const float* src = tile + jj * 128 + (et & 15) * 8;
-              const float4 a0 = *reinterpret_cast<const float4*>(src), a1 = *reinterpret_cast<const float4*>(src + 4);
-              o[t * 8 + 0] = a0.x, o[t * 8 + 1] = a0.y, o[t * 8 + 2] = a0.z, o[t * 8 + 3] = a0.w;
-              o[t * 8 + 4] = a1.x, o[t * 8 + 5] = a1.y, o[t * 8 + 6] = a1.z, o[t * 8 + 7] = a1.w;
-              const long long d_at = static_cast<long long>(out_row0 + jj) * p.ldd + col0;
-              if (b1 != kBinaryNone) r0[t] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.d0) + d_at);
-              if (b2 != kBinaryNone) r1[t] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.d1) + d_at);
-            }
-            if (!pre) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float y = o[i] * p.alpha + bias_v[i & 7];
-                o[i] = u1 == kUnaryRelu ? fmaxf(y, 0.f) : y;
-              }
-            }
-            if (b1 != kBinaryNone) {
-#pragma unroll
-              for (int t = 0; t < 4; ++t) {
-                float f[8];
-                unpack8<BF16>(r0[t], f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[t * 8 + e] = (b1 == kBinaryAdd) ? o[t * 8 + e] + f[e] : o[t * 8 + e] * f[e];
-              }
-            }
-            if (b2 != kBinaryNone) {
-#pragma unroll
-              for (int t = 0; t < 4; ++t) {
-                float f[8];
-                unpack8<BF16>(r1[t], f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[t * 8 + e] = (b2 == kBinaryAdd) ? o[t * 8 + e] + f[e] : o[t * 8 + e] * f[e];
-              }
-            }
-            apply_unary_vec(u2, o);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-              if (j + 8 * t < my_rows)
-                *reinterpret_cast<uint4*>(out0 + row_offset(p, out_row0 + j + 8 * t)) = pack8<BF16>(&o[t * 8]);
-          }
-        }
-        if (!vec) {
-          // columns whose 16-byte accesses are not legal (a ragged last slab, an odd row pitch): element by element
-          for (int j = et >> 4; j < my_rows; j += 8) {
-            const float* src = tile + j * 128 + (et & 15) * 8;
-#pragma unroll 1
-            for (int e = 0; e < 8; ++e)
-              if (col0 + e < p.N) epilogue_scalar_store<BF16>(p, src[e], 0, out_row0 + j, col0 + e);
-          }
-        }
-        // This thread is done reading `partial`: the peers may send the next pass's sums. (Its reads have returned -
-        // their values went into `tile` - so the signal needs no release. A rank without rows signals all the same:
-        // the senders count every peer.)
-        if (R > 1 && !last) {
-#pragma unroll
-          for (int q = 0; q < R; ++q)
-            if (q != rank)
-              mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&partial_taken[seq & 1]), static_cast<uint32_t>(q)));
-        }
-      }
-      }  // passes
-      if (last_slab) break;
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
-    }
-  }
-
-  // Every thread arrives at the cluster-wide barrier exactly once: the epilogue threads did after their last send
-  // (unless a wait ran out first), everybody else does here.
-  if (!epi_arrived) cluster_arrive_relaxed();
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(*tmem_slot, Cfg::kTmemCols);
-  }
-  cluster_wait();  // no CTA leaves while a peer can still write to it or signal it
-}
-
-// One walker per cluster the GPU can hold at once (clusters do not straddle GPCs, so this can be fewer than SMs / R):
-// a cluster left for a second wave would start when the first is already done streaming.
-template <bool BF16, int MX, int R, int H>
-static int swapab_resident_clusters() {
-  using Cfg = SwapCfg<MX, R, H>;
-  static std::atomic<uint64_t> configured{0};
-  static std::atomic<int> resident{0};
-  int clusters = resident.load(std::memory_order_relaxed);
-  if (clusters == 0) {
-    auto* kernel = &gemm_swapab_kernel<BF16, MX, R, H>;
-    opt_in_smem_once(configured, reinterpret_cast<const void*>(kernel), Cfg::kSmemBytes);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(R * (sm_count() / R)));
-    cfg.blockDim = dim3(kSwapThreads);
-    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = R;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    B200AIT_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg));
-    B200AIT_REQUIRE(clusters > 0, "gemm: the weight-streaming kernel's cluster does not fit this GPU");
-    resident.store(clusters, std::memory_order_relaxed);
-  }
-  return clusters;
-}
-
-template <bool BF16, int MX, int R, int H>
-static void launch_swapab(const CUtensorMap& tw, const CUtensorMap& tx, const GemmParams& p, int num_slabs,
-                          int num_groups, cudaStream_t stream) {
-  using Cfg = SwapCfg<MX, R, H>;
-  const int walkers = swapab_resident_clusters<BF16, MX, R, H>();  // also opts the kernel in to its shared memory
-  launch_early(&gemm_swapab_kernel<BF16, MX, R, H>, dim3(static_cast<unsigned>(R * std::min(num_slabs * num_groups, walkers))),
-               kSwapThreads, Cfg::kSmemBytes, stream, true, R, tw, tx, p, num_slabs, num_groups);
-}
-
 // The instantiations the planner chooses from: MX rows of X per group, K split R ways, exchange in H passes.
 struct SwapKernel {
   int mx, r, stages;
   void (*launch)(bool bf16, const CUtensorMap& tw, const CUtensorMap& tx, const GemmParams& p, int num_slabs,
                  int num_groups, cudaStream_t stream);
+  void (*launch_i8)(bool bf16, const CUtensorMap& tw, const CUtensorMap& tx, const GemmParams& p, int num_slabs,
+                    int num_groups, cudaStream_t stream);
   int (*resident)(bool bf16);
 };
 template <int MX, int R, int H>
@@ -810,16 +319,17 @@ static SwapKernel swap_kernel_entry() {
                       else
                         launch_swapab<false, MX, R, H>(tw, tx, p, num_slabs, num_groups, stream);
                     },
+                    &launch_swapab_i8<MX, R, H>,
                     [](bool bf16) {
                       return bf16 ? swapab_resident_clusters<true, MX, R, H>() : swapab_resident_clusters<false, MX, R, H>();
                     }};
 }
 static const std::vector<SwapKernel>& swap_kernels() {
   static const std::vector<SwapKernel> table = {
-      swap_kernel_entry<16, 2, 1>(),  swap_kernel_entry<32, 2, 1>(),  swap_kernel_entry<64, 2, 1>(),
-      swap_kernel_entry<128, 2, 1>(), swap_kernel_entry<256, 2, 2>(), swap_kernel_entry<32, 4, 1>(),
-      swap_kernel_entry<64, 4, 1>(),  swap_kernel_entry<128, 4, 1>(), swap_kernel_entry<256, 4, 2>(),
-      swap_kernel_entry<64, 8, 1>(),  swap_kernel_entry<128, 8, 1>(), swap_kernel_entry<256, 8, 2>()};
+#define B200AIT_SWAP(MX, R, H) swap_kernel_entry<MX, R, H>(),
+      B200AIT_FOR_EACH_SWAP_KERNEL(B200AIT_SWAP)
+#undef B200AIT_SWAP
+  };
   return table;
 }
 
@@ -891,21 +401,26 @@ EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-// 3-D map over a [batch, rows, cols] 16-bit tensor, cols contiguous; box = [1, box_rows, 64], 128-byte swizzle
-CUtensorMap make_tile_map(const void* base, bool bf16, long long cols, long long rows, long long batch,
-                          long long row_stride_elems, long long batch_stride_elems, int box_rows) {
+// 3-D map over a [batch, rows, cols] tensor, cols contiguous; box = [1, box_rows, 128 bytes], 128-byte swizzle
+static CUtensorMap make_box_map(const void* base, CUtensorMapDataType type, int elem_bytes, long long cols, long long rows,
+                                long long batch, long long row_stride_elems, long long batch_stride_elems, int box_rows) {
   CUtensorMap m;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(batch)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_stride_elems) * 2,
-                           static_cast<cuuint64_t>(batch > 1 ? batch_stride_elems : rows * row_stride_elems) * 2};
-  cuuint32_t box[3] = {static_cast<cuuint32_t>(kBK), static_cast<cuuint32_t>(box_rows), 1};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_stride_elems) * elem_bytes,
+                           static_cast<cuuint64_t>(batch > 1 ? batch_stride_elems : rows * row_stride_elems) * elem_bytes};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / elem_bytes), static_cast<cuuint32_t>(box_rows), 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = get_encode_fn()(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                               const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = get_encode_fn()(&m, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw Error("cuTensorMapEncodeTiled failed with CUresult " + std::to_string(static_cast<int>(r)));
   return m;
+}
+
+CUtensorMap make_tile_map(const void* base, bool bf16, long long cols, long long rows, long long batch,
+                          long long row_stride_elems, long long batch_stride_elems, int box_rows) {
+  return make_box_map(base, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, cols, rows, batch,
+                      row_stride_elems, batch_stride_elems, box_rows);
 }
 
 // 5-D map over the GEMM output for the shared-memory-staged store; box = 64 columns x 32 rows,
@@ -943,6 +458,8 @@ struct GemmArgs {
   long long workspace_bytes = 0;
   int split_k = 0;  // 0 = choose, 1 = off, n = at most n splits
   int* status = nullptr;  // device status word to use instead of the library's allocated one
+  int i8 = 0;  // a and b are signed 8-bit integers with a scale per row each (dtype is the result's and the residuals')
+  const float *row_scale = nullptr, *col_scale = nullptr;
 };
 
 constexpr int kTilePair = kGemmPairWidth;  // tile_n value that asks for 256 x 256 tiles on CTA pairs
@@ -1075,6 +592,13 @@ static bool has_own_epilogue(int code) {
   return false;
 }
 
+// the map of an operand whose rows are g.k elements long
+static CUtensorMap operand_map(const GemmArgs& g, const void* base, long long rows, long long batch, long long ld, long long bs,
+                               int box_rows) {
+  if (g.i8) return make_box_map(base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.k, rows, batch, ld, bs, box_rows);
+  return make_tile_map(base, g.dtype == kDTypeBFloat16, g.k, rows, batch, ld, bs, box_rows);
+}
+
 void gemm_run(const GemmArgs& g_in) {
   GemmArgs g = g_in;
   long long c_bdiv = 0, c_bs_hi = 0;
@@ -1109,6 +633,7 @@ void gemm_run(const GemmArgs& g_in) {
   p.lda = g.lda, p.ldb = g.ldb, p.a_bs = g.a_bs, p.b_bs = g.b_bs;
   p.ldc = g.ldc, p.ldd = g.ldd, p.c_bs = g.c_bs, p.d_bs = g.d_bs;
   p.alpha = g.alpha, p.epilogue = g.epilogue;
+  p.row_scale = g.row_scale, p.col_scale = g.col_scale;
   p.store_mode = 0;
   p.t1 = 1, p.t3 = 1, p.d = 1;
   p.c_bdiv = static_cast<int>(c_bdiv), p.c_bs_hi = c_bs_hi;
@@ -1153,15 +678,18 @@ void gemm_run(const GemmArgs& g_in) {
   p.vec_ok = vec ? 1 : 0;
   p.status = g.status ? g.status : device_status_word();
   p.splits = 1;
-  p.kb_per_split = static_cast<int>((g.k + kBK - 1) / kBK);
+  const long long k_block = g.i8 ? kBKOf<true> : kBK;
+  p.kb_per_split = static_cast<int>((g.k + k_block - 1) / k_block);
   p.partial = nullptr;
 
-  const bool tma_ok = (g.k % 8 == 0) && (g.lda % 8 == 0) && (g.ldb % 8 == 0) && aligned16(g.a) && aligned16(g.b) &&
-                      (g.a_bs % 8 == 0) && (g.b_bs % 8 == 0) && g.batch < 65536 * 32;
+  // (8-bit operands of any K: boxes end in zeros past it, and the copy needs no more than the pitch and the address)
+  const bool tma_ok = g.i8 ? g.lda % 16 == 0 && g.ldb % 16 == 0 && aligned16(g.a) && aligned16(g.b)
+                           : (g.k % 8 == 0) && (g.lda % 8 == 0) && (g.ldb % 8 == 0) && aligned16(g.a) && aligned16(g.b) &&
+                                 (g.a_bs % 8 == 0) && (g.b_bs % 8 == 0) && g.batch < 65536 * 32;
   B200AIT_REQUIRE(tma_ok || g.num_out == 1, "gemm: several output buffers need TMA-addressable operands");
   // M <= 4, deep K, the caller left tile width and split-K to the library: stream W once on the CUDA cores
   const long long rowdot_smem = (g.m <= 1 ? 1 : g.m <= 2 ? 2 : 4) * g.k * 2;
-  if (tma_ok && g.batch == 1 && !g.b_mn && g.num_out == 1 && g.tile_n == 0 && g.split_k == 0 &&
+  if (tma_ok && !g.i8 && g.batch == 1 && !g.b_mn && g.num_out == 1 && g.tile_n == 0 && g.split_k == 0 &&
       gemm_rowdot_long(g.m, g.n, g.k)) {
     const unsigned grid = static_cast<unsigned>(std::min<long long>(sm_count(), (g.n + 3) / 4));
     const int smem = static_cast<int>(rowdot_smem);
@@ -1182,7 +710,7 @@ void gemm_run(const GemmArgs& g_in) {
   }
   // the same for shorter rows, where they are not too many (rules.h); below K = 256 the tile kernels are level or ahead (K =
   // 128, N = 8192: 4.8 against 3.1 .. 6.0 us)
-  if (tma_ok && g.batch == 1 && g.m <= kRowDotMaxM && !g.b_mn && g.num_out == 1 && g.tile_n == 0 && g.split_k == 0 &&
+  if (tma_ok && !g.i8 && g.batch == 1 && g.m <= kRowDotMaxM && !g.b_mn && g.num_out == 1 && g.tile_n == 0 && g.split_k == 0 &&
       gemm_rowdot_short(g.m, g.n, g.k, p.vec_ok != 0, bf16)) {
     const unsigned grid = static_cast<unsigned>(std::min<long long>(sm_count(), (g.n + 3) / 4));
 #define B200AIT_ROWDOT(MR, KV)                                                                                    \
@@ -1208,13 +736,15 @@ void gemm_run(const GemmArgs& g_in) {
   // few rows of X, or few output tiles: the weight-streaming kernel where its planner takes the problem
   const bool streams = tma_ok && g.batch == 1 && !g.b_mn && g.num_out == 1 && g.tile_n == 0 && g.split_k == 0;
   // (row-major B: its boxes are not rows of K, and the figures of rules.h do not hold)
-  const long long pitch = g.b_mn ? kBK : gemm_copy_row_us(g.lda) > gemm_copy_row_us(g.ldb) ? g.lda : g.ldb;
-  GemmProblem problem{g.batch, g.m, g.n, g.k, 0, 0, pitch, g.b_mn || g.num_out > 1};
+  // (8-bit operands count as 16-bit ones of half the length: the estimates are about boxes of 128 bytes and their MMAs)
+  const long long lda = g.i8 ? g.lda / 2 : g.lda, ldb = g.i8 ? g.ldb / 2 : g.ldb, k16 = g.i8 ? (g.k + 1) / 2 : g.k;
+  const long long pitch = g.b_mn ? kBK : gemm_copy_row_us(lda) > gemm_copy_row_us(ldb) ? lda : ldb;
+  GemmProblem problem{g.batch, g.m, g.n, k16, 0, 0, pitch, g.b_mn || g.num_out > 1};
   // CTA pairs do not write permuted batches, and with an epilogue read from the parameters (two residuals, an activation without an
   // instantiation of its own) they need K to hide it behind: 829 x 6824 x 216 + add + add 23.6 us, 128-wide tiles 17.9, 1234 x 4768 x 72
   // mul_tanh 19.7 and 15.0. Over 260 problems with such epilogues, from K = 512 on none is slower than by the rule of whole waves before.
   const bool own_epilogue = has_own_epilogue(p.epilogue) && (b1 != kBinaryNone || p.alpha == 1.f);
-  problem.pairs = p.c_bdiv == 0 && (g.batch > 1 || own_epilogue || g.k >= 512);
+  problem.pairs = p.c_bdiv == 0 && (g.batch > 1 || own_epilogue || k16 >= 512);
   GemmPlan planned{g.tile_n, nullptr};
   {
     const int code = p.epilogue;
@@ -1230,9 +760,9 @@ void gemm_run(const GemmArgs& g_in) {
     if (const SwapKernel* sk = planned.swap) {
       const int num_groups = static_cast<int>((g.m + sk->mx - 1) / sk->mx);
       const int num_slabs = static_cast<int>((g.n + 127) / 128);
-      CUtensorMap tw = make_tile_map(g.b, bf16, g.k, g.n, 1, g.ldb, 0, 128);
-      CUtensorMap tx = make_tile_map(g.a, bf16, g.k, g.m, 1, g.lda, 0, sk->mx);
-      sk->launch(bf16, tw, tx, p, num_slabs, num_groups, g.stream);
+      CUtensorMap tw = operand_map(g, g.b, g.n, 1, g.ldb, 0, 128);
+      CUtensorMap tx = operand_map(g, g.a, g.m, 1, g.lda, 0, sk->mx);
+      (g.i8 ? sk->launch_i8 : sk->launch)(bf16, tw, tx, p, num_slabs, num_groups, g.stream);
       return;
     }
   }
@@ -1240,10 +770,15 @@ void gemm_run(const GemmArgs& g_in) {
     dim3 grid(static_cast<unsigned>((g.n + 31) / 32), static_cast<unsigned>((g.m + 31) / 32),
               static_cast<unsigned>(g.batch));
     B200AIT_REQUIRE(grid.y < 65536 && grid.z < 65536, "gemm: unaligned problem too large for the CUDA-core kernel");
-    if (bf16)
-      ::b200ait::count_launch(), gemm_simt_kernel<true><<<grid, 256, 0, g.stream>>>(g.a, g.b, p);
+    count_launch();
+    if (g.i8 && bf16)
+      gemm_simt_i8_kernel<true><<<grid, 256, 0, g.stream>>>(static_cast<const int8_t*>(g.a), static_cast<const int8_t*>(g.b), p);
+    else if (g.i8)
+      gemm_simt_i8_kernel<false><<<grid, 256, 0, g.stream>>>(static_cast<const int8_t*>(g.a), static_cast<const int8_t*>(g.b), p);
+    else if (bf16)
+      gemm_simt_kernel<true><<<grid, 256, 0, g.stream>>>(g.a, g.b, p);
     else
-      ::b200ait::count_launch(), gemm_simt_kernel<false><<<grid, 256, 0, g.stream>>>(g.a, g.b, p);
+      gemm_simt_kernel<false><<<grid, 256, 0, g.stream>>>(g.a, g.b, p);
     B200AIT_CUDA_CHECK(cudaGetLastError());
     return;
   }
@@ -1252,7 +787,7 @@ void gemm_run(const GemmArgs& g_in) {
                   "gemm: tile_n must be 64, 128, 256 or 512 (256 x 256 tiles on CTA pairs)");
   const bool ws_ok = g.workspace != nullptr && aligned16(g.workspace);
   const bool force_pair = g.tile_n == kTilePair;
-  SplitPlan sp = force_pair ? SplitPlan{kTilePair, 1, static_cast<int>((g.k + kBK - 1) / kBK), 0}
+  SplitPlan sp = force_pair || g.i8 ? SplitPlan{g.tile_n ? g.tile_n : planned.tile_n, 1, p.kb_per_split, 0}
                             : plan_split_k(problem, g.tile_n, planned.tile_n, g.num_out > 1 ? 1 : g.split_k, ws_ok ? g.workspace_bytes : 0,
                                            streams);
   if (g.num_out > 1 && sp.tile_n == 64 && g.tile_n == 0) sp.tile_n = 128;  // several destinations need the staged store
@@ -1265,9 +800,9 @@ void gemm_run(const GemmArgs& g_in) {
   p.kb_per_split = sp.kb_per_split;
   p.partial = static_cast<float*>(g.workspace);
   const long long a_batch = p.a_batch_mul ? g.batch : 1, b_batch = p.b_batch_mul ? g.batch : 1;
-  CUtensorMap ta = make_tile_map(g.a, bf16, g.k, g.m, a_batch, g.lda, g.a_bs, kBM);
+  CUtensorMap ta = operand_map(g, g.a, g.m, a_batch, g.lda, g.a_bs, kBM);
   CUtensorMap tb = g.b_mn ? make_tile_map(g.b, bf16, g.n, g.k, b_batch, g.ldb, g.b_bs, kBK)  // 64 x 64 boxes
-                          : make_tile_map(g.b, bf16, g.k, g.n, b_batch, g.ldb, g.b_bs, pair ? bn / 2 : bn);
+                          : operand_map(g, g.b, g.n, b_batch, g.ldb, g.b_bs, pair ? bn / 2 : bn);
   // Staged TMA store: row-major output with 16-byte aligned rows, or a permuted output whose 64-column
   // groups and 32-row groups each stay inside one contiguous run of the destination.
   OutMaps tout;
@@ -1309,7 +844,7 @@ void gemm_run(const GemmArgs& g_in) {
   const FastDiv by_batch(p.tiles_m * p.tiles_n), by_group(kGroupM * p.tiles_n), by_rest(std::max(1, p.tiles_m % kGroupM));
   p.batch_mul = by_batch.mul, p.batch_shr = by_batch.shr, p.group_mul = by_group.mul, p.group_shr = by_group.shr;
   p.rest_mul = by_rest.mul, p.rest_shr = by_rest.shr;
-  p.ring_limit = operand_ring_limit(g.k);
+  p.ring_limit = operand_ring_limit(k16);
   const int grid = pair ? 2 * std::min(p.num_units, sm_count() / 2) : std::min(p.num_units, sm_count());
   CUtensorMap td0 = ta;
   p.tma_d0 = 0;
@@ -1318,7 +853,11 @@ void gemm_run(const GemmArgs& g_in) {
     td0 = make_tile_map(g.d0, bf16, g.n, g.m, g.batch, g.ldd, g.d_bs, 32);
     p.tma_d0 = 1;
   }
-  if (pair)
+  if (g.i8 && bf16)
+    launch_tc_i8<true>(sp.tile_n, ta, tb, tout, td0, p, grid, g.stream);
+  else if (g.i8)
+    launch_tc_i8<false>(sp.tile_n, ta, tb, tout, td0, p, grid, g.stream);
+  else if (pair)
     launch_tc_pair256(bf16, ta, tb, tout, td0, p, grid, g.stream);
   else if (bn == 256)
     launch_tc_width<256>(bf16, ta, tb, tout, p, grid, g.stream);
@@ -1358,6 +897,25 @@ B200AIT_EXPORT int b200ait_gemm_rcr(const void* a, const void* b, const void* bi
     g.workspace = workspace;
     g.workspace_bytes = workspace_bytes;
     g.split_k = split_k;
+    gemm_run(g);
+  });
+}
+
+// gemm_rcr of signed 8-bit integers: c = epilogue(sum_k a[m, k] b[n, k] * a_scale[m] * b_scale[n] + bias, d0, d1).
+B200AIT_EXPORT int b200ait_gemm_rcr_i8(const void* a, const float* a_scale, const void* b, const float* b_scale,
+                                       const void* bias, const void* d0, const void* d1, void* c, int64_t m, int64_t n,
+                                       int64_t k, int64_t lda, int64_t ldb, int64_t ldc, int64_t ldd, int epilogue, int dtype,
+                                       int tile_n, cudaStream_t stream) {
+  return guarded("b200ait_gemm_rcr_i8", [&] {
+    // sums of K products of at most 2^14 each stay below 2^31
+    B200AIT_REQUIRE(k < (1 << 17), "gemm: 8-bit operands take up to 131071 columns");
+    B200AIT_REQUIRE(m <= 0 || n <= 0 || k != 0, "gemm: 8-bit operands have no columns");
+    B200AIT_REQUIRE(m <= 0 || n <= 0 || k <= 0 || (lda >= k && ldb >= k && ldc >= n), "gemm: a row pitch is shorter than the row");
+    const int b1 = epi_b1(epilogue), b2 = epi_b2(epilogue);
+    B200AIT_REQUIRE((b1 == kBinaryNone && b2 == kBinaryNone) || ldd >= n, "gemm: a row pitch is shorter than the row");
+    GemmArgs g{a, b, bias, d0, d1, c, 1, m, n, k, lda, ldb, ldc, ldd, 0, 0, 0, 0, epilogue, dtype, 1.f, 0, 1, 1, 1, tile_n, stream};
+    if (m > 0 && n > 0 && k > 0) B200AIT_REQUIRE(a_scale && b_scale, "gemm: 8-bit operands need the scales of their rows");
+    g.i8 = 1, g.row_scale = a_scale, g.col_scale = b_scale;
     gemm_run(g);
   });
 }

@@ -46,6 +46,9 @@ struct GemmParams {
   // 0 = plain batch stride. Only the kernels with a run-time epilogue (EPI < 0) and the CUDA-core kernel honour it.
   int c_bdiv;
   long long c_bs_hi;
+  // operands of signed 8-bit integers: y = epilogue(sum * col_scale[col] * row_scale[row] + bias); null otherwise
+  const float* row_scale;  // [M]
+  const float* col_scale;  // [N]
 };
 
 // Tensor maps of the output: one per destination buffer. More than one destination is how a rank that owns a
@@ -56,7 +59,11 @@ struct OutMaps {
 };
 
 constexpr int kBM = 128;
-constexpr int kBK = 64;
+constexpr int kBK = 64;  // 16-bit elements of a k-block: 128 bytes of a row, four MMAs
+// ... of either type. A k-block of 8-bit integers is the same 128 bytes, in the same boxes and for the same four MMAs, which
+// multiply twice as many of them.
+template <bool I8>
+constexpr int kBKOf = I8 ? 2 * kBK : kBK;
 constexpr int kGroupM = 8;  // row blocks whose tiles run side by side
 constexpr int kEpiWarps = 8;                      // two per TMEM lane quarter, each takes half of the columns
 constexpr int kGemmThreads = 64 + 32 * kEpiWarps;  // producer warp + MMA warp + epilogue warps
@@ -69,7 +76,9 @@ constexpr int kGemmThreads = 64 + 32 * kEpiWarps;  // producer warp + MMA warp +
 // ROWS: the output is written row by row from staging boxes, which 64-wide tiles do not have otherwise: their 32 KB come
 // out of the L1 cache, and the other kernels' per-thread residual loads want it (32768 x 41 x 320 with two residuals: 22.3
 // us, 24.7 beside idle boxes).
-template <int BN, bool PAIR = false, bool D0BOX = false, bool ROWS = false>
+// I8: the columns' scales lie in shared memory beside the bias. With 256 columns that leaves room for one tile's of each, where the
+// other kernels keep two.
+template <int BN, bool PAIR = false, bool D0BOX = false, bool ROWS = false, bool I8 = false>
 struct TileCfg {
   static_assert(!D0BOX || PAIR, "staged residual boxes are only built for the CTA-pair tile");
   static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B rows this CTA loads per stage
@@ -79,8 +88,9 @@ struct TileCfg {
   static constexpr int kBoxesPerWarp = D0BOX ? 2 : 1;  // 32 rows x 64 columns x 16 bit = 4 KB each
   static constexpr int kStagingBytes = (BN >= 128 || ROWS) ? kEpiWarps * kBoxesPerWarp * 4096 : 0;
   static constexpr int kBarrierBytes = 512;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kBarrierBytes +
-                                    2 * BN * 4 /*bias tile, fp32, one per accumulator*/;
+  static constexpr int kVectors = I8 && BN == 256 ? 1 : 2;  // bias tiles (fp32): one per accumulator, or one
+  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kBarrierBytes + (I8 ? 2 : 1) * kVectors * BN * 4;
+  static_assert(kSmemBytes <= 227 * 1024, "tile kernel: shared memory");
 };
 
 // EPI of the instantiations that read the epilogue from the parameters and write the output row by row (the plain
@@ -216,6 +226,40 @@ __device__ __forceinline__ void epilogue_chunk32(const GemmParams& p, float (&v)
   }
 }
 
+// What follows the bias in the fused epilogue of one element, and its store: activation, residual(s), activation, one rounding.
+template <bool BF16>
+__device__ __forceinline__ void epilogue_scalar_rest(const GemmParams& p, float v, int b, int row, int col) {
+  using E = Elem16<BF16>;
+  using T = typename E::T;
+  const int u1 = epi_u1(p.epilogue), b1 = epi_b1(p.epilogue), b2 = epi_b2(p.epilogue), u2 = epi_u2(p.epilogue);
+  v = apply_unary(u1, v);
+  const long long di = static_cast<long long>(b) * p.d_bs + static_cast<long long>(row) * p.ldd + col;
+  if (b1 != kBinaryNone) {
+    const float f = E::to_float(static_cast<const T*>(p.d0)[di]);
+    v = (b1 == kBinaryAdd) ? v + f : v * f;
+  }
+  if (b2 != kBinaryNone) {
+    const float f = E::to_float(static_cast<const T*>(p.d1)[di]);
+    v = (b2 == kBinaryAdd) ? v + f : v * f;
+  }
+  v = apply_unary(u2, v);
+  static_cast<T*>(p.out)[batch_offset(p, b) + row_offset(p, row) + col_offset(p, col)] = E::from_float(v);
+}
+// The fused epilogue on one fp32 accumulator: alpha, bias and the rest.
+template <bool BF16>
+__device__ __forceinline__ void epilogue_scalar_store(const GemmParams& p, float acc, int b, int row, int col) {
+  float v = acc * p.alpha;
+  if (p.bias) v += Elem16<BF16>::to_float(static_cast<const typename Elem16<BF16>::T*>(p.bias)[col]);
+  epilogue_scalar_rest<BF16>(p, v, b, row, col);
+}
+// The same on a sum of 8-bit products times its column's scale, rounded as the tile kernels round.
+template <bool BF16>
+__device__ __forceinline__ void epilogue_scalar_store_i8(const GemmParams& p, float scaled, int row, int col) {
+  const float rs = p.row_scale[row];
+  const float v = p.bias ? __fmaf_rn(scaled, rs, Elem16<BF16>::to_float(static_cast<const typename Elem16<BF16>::T*>(p.bias)[col]))
+                         : scaled * rs;
+  epilogue_scalar_rest<BF16>(p, v, 0, row, col);
+}
 
 // EPI >= 0 fixes the epilogue code at compile time (straight-line code for the common epilogues);
 // EPI < 0 reads it from the parameters.
@@ -388,10 +432,12 @@ __device__ __forceinline__ void store_box_rows(const GemmParams& p, const uint8_
   }
 }
 
+// I8: operands of signed 8-bit integers with a scale per row of A and per row of B (p.row_scale, p.col_scale), 32-bit integer sums,
+// results in 16 bits. Sums are exact, so a result does not depend on the tile or on how K is shared out.
 // BMN: B is stored [K, N]. MULTI: the staged store goes to p.num_out destinations. Both are compile-time, so that
 // the plain [N, K] single-destination kernels carry no trace of them (a run-time flag cost the BERT-layer GEMMs
 // 2-3 %), and both are only instantiated with the generic epilogue (EPI == -1).
-template <int BN, bool BF16, int EPI, bool PAIR, bool BMN = false, bool MULTI = false>
+template <int BN, bool BF16, int EPI, bool PAIR, bool BMN = false, bool MULTI = false, bool I8 = false>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                const __grid_constant__ CUtensorMap tma_out, const __grid_constant__ CUtensorMap tma_d0,
@@ -399,7 +445,9 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
   // `tma_out` is the (first) destination; `outs.m[1..]` are the extra destinations of a multi-destination store
   // and sit at the end of the parameter space, out of the way of what every launch reads.
   constexpr bool D0BOX = d0_box_of<EPI, PAIR>();
-  using Cfg = TileCfg<BN, PAIR, D0BOX, EPI == kRowsEpilogue>;
+  using Cfg = TileCfg<BN, PAIR, D0BOX, EPI == kRowsEpilogue, I8>;
+  static_assert(!I8 || (!BMN && !MULTI), "8-bit operands: [N, K] storage, one destination");
+  constexpr int kBKE = kBKOf<I8>;
   constexpr int kStages = Cfg::kStages;
   const int ring = min(kStages, p.ring_limit);
   constexpr uint32_t kABytes = kBM * kBK * 2;
@@ -415,7 +463,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
   // alpha = 1, no split-K, the staged store and (with a residual: CTA pairs only) staged residual boxes. Their
   // code carries none of the other paths, which is worth several per cent on the short-K GEMMs.
   constexpr bool kLean = EPI >= 0 && BN >= 128 && (PAIR || epi_b1(EPI < 0 ? 0 : EPI) == kBinaryNone);
-  const int splits = (PAIR || kLean) ? 1 : p.splits;  // CTA pairs never split K either
+  const int splits = (PAIR || kLean || I8) ? 1 : p.splits;  // CTA pairs and 8-bit operands never split K either
   // Work distribution: a single CTA, or a pair of CTAs (cluster ranks 0 and 1), walks the units.
   const int pair_rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
   const int walker = PAIR ? (blockIdx.x >> 1) : blockIdx.x;
@@ -430,11 +478,11 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d0_bar + 2 * kEpiWarps);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   static_assert((2 * kStages + 5 + 2 * kEpiWarps) * 8 + 8 <= Cfg::kBarrierBytes, "barrier area too small");
-  float* sbias = reinterpret_cast<float*>(staging + Cfg::kStagingBytes + Cfg::kBarrierBytes);  // [2][BN]
+  float* sbias = reinterpret_cast<float*>(staging + Cfg::kStagingBytes + Cfg::kBarrierBytes);  // [kVectors][BN]
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // known to be uniform
   const int lane = threadIdx.x & 31;
-  const int num_kb = (p.K + kBK - 1) / kBK;
+  const int num_kb = (p.K + kBKE - 1) / kBKE;
 
   // unit of work -> tile and K share (only the plain kernels split K)
   auto split_unit = [&](int unit, int& tile, int& split) {
@@ -517,23 +565,23 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
         const uint32_t bar = full0_of_leader + static_cast<uint32_t>(stage) * 8u;
         if (PAIR) {
           if (pair_rank == 0) mbar_arrive_expect_tx_warp(&full_bar[stage], 2 * kStageBytes, lead);
-          tma_load_3d_pair_warp(sa, &tma_a, bar, kb * kBK, m0, a_b, lead);
+          tma_load_3d_pair_warp(sa, &tma_a, bar, kb * kBKE, m0, a_b, lead);
           if (BMN) {  // [K, N] storage: one box of 64 k-rows x 64 columns per 64-column chunk
 #pragma unroll
             for (int ch = 0; ch < Cfg::kBRows / 64; ++ch)
-              tma_load_3d_pair_warp(sb + ch * 8192, &tma_b, bar, n0 + ch * 64, kb * kBK, b_b, lead);
+              tma_load_3d_pair_warp(sb + ch * 8192, &tma_b, bar, n0 + ch * 64, kb * kBKE, b_b, lead);
           } else {
-            tma_load_3d_pair_warp(sb, &tma_b, bar, kb * kBK, n0, b_b, lead);
+            tma_load_3d_pair_warp(sb, &tma_b, bar, kb * kBKE, n0, b_b, lead);
           }
         } else {
           mbar_arrive_expect_tx_warp(&full_bar[stage], kStageBytes, lead);
-          tma_load_3d_warp(sa, &tma_a, bar, kb * kBK, m0, a_b, lead);
+          tma_load_3d_warp(sa, &tma_a, bar, kb * kBKE, m0, a_b, lead);
           if (BMN) {
 #pragma unroll
             for (int ch = 0; ch < Cfg::kBRows / 64; ++ch)
-              tma_load_3d_warp(sb + ch * 8192, &tma_b, bar, n0 + ch * 64, kb * kBK, b_b, lead);
+              tma_load_3d_warp(sb + ch * 8192, &tma_b, bar, n0 + ch * 64, kb * kBKE, b_b, lead);
           } else {
-            tma_load_3d_warp(sb, &tma_b, bar, kb * kBK, n0, b_b, lead);
+            tma_load_3d_warp(sb, &tma_b, bar, kb * kBKE, n0, b_b, lead);
           }
         }
         if (++stage == ring) {
@@ -565,7 +613,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
     // -------------------------------------------------------------- MMA issuer
     const uint32_t tmem_base = *tmem_slot;
     if (pair_rank == 0) {
-      constexpr uint32_t idesc = umma_idesc_f16(PAIR ? 2 * kBM : kBM, BN, BF16, false, BMN);
+      constexpr int kMmaM = PAIR ? 2 * kBM : kBM;
+      constexpr uint32_t idesc = I8 ? umma_idesc_i8(kMmaM, BN) : umma_idesc_f16(kMmaM, BN, BF16, false, BMN);
       const uint32_t lead = elect_one();
       int stage = 0;
       uint32_t phase = 0;
@@ -593,7 +642,11 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k) {
             const uint32_t accumulate = (kb > kb0 || k != 0) ? 1u : 0u;
-            if (PAIR) {
+            if constexpr (I8 && PAIR) {
+              umma_i8_ss_pair_warp(d_tmem, a_lo + k * (32 >> 4), b_lo + k * kBStep, idesc, accumulate, lead);
+            } else if constexpr (I8) {
+              umma_i8_ss_warp(d_tmem, a_lo + k * (32 >> 4), b_lo + k * kBStep, idesc, accumulate, lead);
+            } else if (PAIR) {
               umma_f16_ss_pair_warp(d_tmem, a_lo + k * (32 >> 4), b_lo + k * kBStep, idesc, accumulate, lead);
             } else {
               umma_f16_ss_warp(d_tmem, a_lo + k * (32 >> 4), b_lo + k * kBStep, idesc, accumulate, lead);
@@ -682,16 +735,20 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
           }
         }
       }
-      float* bias_s = sbias + acc * BN;
-      if (has_bias) {  // CTA-uniform
+      float* bias_s = sbias + (Cfg::kVectors == 2 ? acc * BN : 0);
+      float* scale_s = bias_s + Cfg::kVectors * BN;  // I8 only
+      if (I8 || has_bias) {  // CTA-uniform
+        if (Cfg::kVectors == 1) named_bar_sync(1, 32 * kEpiWarps);  // every warp is done with the last tile's
         if (et < BN) {
           const int col = n_blk * BN + et;
-          bias_s[et] = col < p.N ? E::to_float(static_cast<const T*>(p.bias)[col]) : 0.f;
+          if (!I8 || has_bias) bias_s[et] = col < p.N ? E::to_float(static_cast<const T*>(p.bias)[col]) : 0.f;
+          if (I8) scale_s[et] = col < p.N ? p.col_scale[col] : 0.f;
         }
         named_bar_sync(1, 32 * kEpiWarps);
       }
       const int row = m_blk * kBM + quarter * 32 + lane;
       const bool row_ok = row < p.M;
+      const float row_scale = I8 && row_ok ? p.row_scale[row] : 0.f;
       const T* d0_row = static_cast<const T*>(p.d0) + static_cast<long long>(b) * p.d_bs + static_cast<long long>(row) * p.ldd;
       uint4 d0v[4];
       auto prefetch_d0 = [&](int col0) {
@@ -735,7 +792,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
         if (col0 >= p.N) return;  // warp-uniform
         float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(cur[j]);
+        for (int j = 0; j < 32; ++j) v[j] = I8 ? __int2float_rn(static_cast<int>(cur[j])) : __uint_as_float(cur[j]);
         const bool full = p.vec_ok && (col0 + 32 <= p.N);
         if (splits > 1) {
           // split-K: raw fp32 partial sums; the reduce kernel applies the epilogue
@@ -753,11 +810,25 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
           }
           return;
         }
-        if (!kLean && p.alpha != 1.f) {
+        if constexpr (I8) {
+          const float* cs = scale_s + half * (BN / 2) + c * 32;
+          const uint64_t rs = pack2(row_scale, row_scale);
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const float2 f = *reinterpret_cast<const float2*>(cs + q * 2);
+            const uint64_t x = mul2(pack2(v[q * 2], v[q * 2 + 1]), pack2(f.x, f.y));
+            if (has_bias) {
+              const float2 g = *reinterpret_cast<const float2*>(bias_s + half * (BN / 2) + c * 32 + q * 2);
+              unpack2(fma2(x, rs, pack2(g.x, g.y)), v[q * 2], v[q * 2 + 1]);
+            } else {
+              unpack2(mul2(x, rs), v[q * 2], v[q * 2 + 1]);
+            }
+          }
+        } else if (!kLean && p.alpha != 1.f) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= p.alpha;
         }
-        if (has_bias) {
+        if (!I8 && has_bias) {
           const float* bs = bias_s + half * (BN / 2) + c * 32;
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
@@ -872,24 +943,24 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
   }
 }
 
-template <int BN, bool BF16, int EPI, bool BMN = false, bool MULTI = false>
+template <int BN, bool BF16, int EPI, bool BMN = false, bool MULTI = false, bool I8 = false>
 void launch_tc(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& tout, const GemmParams& p, int grid,
                cudaStream_t stream) {
-  using Cfg = TileCfg<BN, false, false, EPI == kRowsEpilogue>;
+  using Cfg = TileCfg<BN, false, false, EPI == kRowsEpilogue, I8>;
   static std::atomic<uint64_t> configured{0};
-  opt_in_smem_once(configured, reinterpret_cast<const void*>(&gemm_tc_kernel<BN, BF16, EPI, false, BMN, MULTI>),
+  opt_in_smem_once(configured, reinterpret_cast<const void*>(&gemm_tc_kernel<BN, BF16, EPI, false, BMN, MULTI, I8>),
                    Cfg::kSmemBytes);
-  launch_early(&gemm_tc_kernel<BN, BF16, EPI, false, BMN, MULTI>, dim3(static_cast<unsigned>(grid)), kGemmThreads, Cfg::kSmemBytes,
+  launch_early(&gemm_tc_kernel<BN, BF16, EPI, false, BMN, MULTI, I8>, dim3(static_cast<unsigned>(grid)), kGemmThreads, Cfg::kSmemBytes,
                stream, gemm_starts_early(p.num_units, grid, p.tma_store, sm_count()), 1, ta, tb, tout.m[0], ta, p, tout);
 }
 
 // CTA-pair variant: `grid` counts CTAs (twice the number of pairs); launched as clusters of two.
-template <int BN, bool BF16, int EPI, bool BMN = false, bool MULTI = false>
+template <int BN, bool BF16, int EPI, bool BMN = false, bool MULTI = false, bool I8 = false>
 void launch_tc_pair(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& tout, const CUtensorMap& td0,
                     const GemmParams& p, int grid, cudaStream_t stream) {
-  using Cfg = TileCfg<BN, true, d0_box_of<EPI, true>(), EPI == kRowsEpilogue>;
+  using Cfg = TileCfg<BN, true, d0_box_of<EPI, true>(), EPI == kRowsEpilogue, I8>;
   static std::atomic<uint64_t> configured{0};
-  auto* kernel = &gemm_tc_kernel<BN, BF16, EPI, true, BMN, MULTI>;
+  auto* kernel = &gemm_tc_kernel<BN, BF16, EPI, true, BMN, MULTI, I8>;
   opt_in_smem_once(configured, reinterpret_cast<const void*>(kernel), Cfg::kSmemBytes);
   launch_early(kernel, dim3(static_cast<unsigned>(grid)), kGemmThreads, Cfg::kSmemBytes, stream,
                gemm_starts_early(p.num_units, grid / 2, p.tma_store, sm_count()), 2, ta, tb, tout.m[0], td0, p, tout);
@@ -938,6 +1009,17 @@ void launch_tc_pair256(bool bf16, const CUtensorMap& ta, const CUtensorMap& tb, 
 
 void launch_tc_pair256_bf16_lean(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& tout,
                                  const CUtensorMap& td0, const GemmParams& p, int grid, cudaStream_t stream);
+
+// 8-bit operands; width 64, 128, 256 or kGemmPairWidth. Defined in gemm_i8.cu and gemm_i8_bf16.cu.
+template <bool BF16>
+void launch_tc_i8(int width, const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& tout, const CUtensorMap& td0,
+                  const GemmParams& p, int grid, cudaStream_t stream);
+template <>
+void launch_tc_i8<false>(int, const CUtensorMap&, const CUtensorMap&, const OutMaps&, const CUtensorMap&, const GemmParams&, int,
+                         cudaStream_t);
+template <>
+void launch_tc_i8<true>(int, const CUtensorMap&, const CUtensorMap&, const OutMaps&, const CUtensorMap&, const GemmParams&, int,
+                        cudaStream_t);
 
 #define B200AIT_DEFINE_LAUNCH_TC_WIDTH(BN_)                                                                    \
   template <>                                                                                                  \

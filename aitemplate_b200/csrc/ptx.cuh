@@ -214,6 +214,17 @@ __device__ __forceinline__ void umma_f16_ss_warp(uint32_t d_tmem, uint32_t a_lo,
       "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kUmmaDescHiSw128), "r"(lead)
       : "memory");
 }
+// the same for 8-bit integers, 32 of them per row and instruction, with 32-bit sums
+__device__ __forceinline__ void umma_i8_ss_warp(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
+                                                uint32_t accumulate, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kUmmaDescHiSw128), "r"(lead)
+      : "memory");
+}
 // D[tmem] (+)= A[tmem] * B[smem]
 __device__ __forceinline__ void umma_f16_ts_warp(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc,
                                                  uint32_t accumulate, uint32_t lead) {
@@ -323,6 +334,16 @@ __device__ __forceinline__ void umma_f16_ss_pair_warp(uint32_t d_tmem, uint32_t 
       "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kUmmaDescHiSw128), "r"(lead)
       : "memory");
 }
+__device__ __forceinline__ void umma_i8_ss_pair_warp(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
+                                                     uint32_t accumulate, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kUmmaDescHiSw128), "r"(lead)
+      : "memory");
+}
 // one arrival on the mbarrier at this shared-memory offset in every CTA of `cta_mask`
 __device__ __forceinline__ void umma_commit_pair_warp(uint64_t* bar, uint16_t cta_mask, uint32_t lead) {
   asm volatile(
@@ -341,6 +362,11 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, bool bf16, b
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn_major ? 1u : 0u) << 15) |
          ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// The same for kind::i8, both operands signed and K-major: D format 2 = s32, A and B format 1 = signed 8 bits.
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
 // TMEM -> registers: this warp's 32 lanes x 32 consecutive 32-bit columns (one row per thread)

@@ -385,6 +385,186 @@ def flash_attention(qkv: torch.Tensor, cu_seqlens: torch.Tensor, max_seq_len: in
     return out
 
 
+def _check_here(what: str, **tensors) -> None:
+    """The operands of a call whose kernels are told apart by type: CUDA tensors of the current device."""
+    here = torch._C._cuda_getDevice()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{what}: {name} must be a CUDA tensor")
+        if t.device.index != here:
+            raise ValueError(f"{what}: {name} is on cuda:{t.device.index}, the current device is cuda:{here}")
+
+
+def _row_pitch(what: str, name: str, t: torch.Tensor) -> int:
+    """Elements from row to row of a tensor that is read as rows of its last dim."""
+    if t.dim() < 1 or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{what}: the elements of a row of {name} must lie side by side")
+    n, pitch, step = t.shape[-1], None, None
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] == 1:
+            continue
+        if pitch is None:
+            pitch = t.stride(d)
+        elif t.stride(d) != step:
+            raise ValueError(f"{what}: the rows of {name} must lie at one distance")
+        step = t.stride(d) * t.shape[d]
+    if pitch is None:  # a single row
+        return n
+    if pitch < n and t.numel():
+        raise ValueError(f"{what}: the rows of {name} overlap")
+    return pitch
+
+
+def _padded(n: int) -> int:
+    return (n + 15) // 16 * 16
+
+
+def _int8_rows(like: torch.Tensor, lead: Sequence[int], n: int) -> torch.Tensor:
+    """An uninitialised int8 [*lead, n] whose rows start on 16 bytes, as the tensor cores want them."""
+    if n % 16 == 0:
+        return torch.empty([*lead, n], dtype=torch.int8, device=like.device)
+    return torch.empty([*lead, _padded(n)], dtype=torch.int8, device=like.device)[..., :n]
+
+
+def quantize_rows(x: torch.Tensor, activation: str = "identity", gated: bool = False):
+    """(q, scale): the rows (last dim) of act(x) as int8 with an fp32 scale each, the left operand of gemm_rcr_i8.
+    scale = max |v| / 127, q = round(127 v / max |v|), ties to even. With `gated` x holds the two halves of a gated
+    feed-forward's first product, and v = act(x[..., :n]) * x[..., n:]. A row of zeros gets scale 0; a row with an infinity or
+    a NaN in it gets scale NaN and zeros. Rows of x may lie apart. Where n is not a multiple of 16, q is a view of rows padded
+    to 16 bytes, so that the product can read them with the tensor cores."""
+    _check_here("quantize_rows", x=x)
+    if activation not in UNARY:
+        raise ValueError(f"quantize_rows: unknown activation {activation}")
+    pitch = _row_pitch("quantize_rows", "x", x)
+    n = x.shape[-1]
+    if gated:
+        if n % 2:
+            raise ValueError(f"quantize_rows: the rows of a gated x have two halves, got {n} columns")
+        n //= 2
+    if n == 0:
+        raise ValueError("quantize_rows: x has no columns")
+    lead = x.shape[:-1]
+    q = _int8_rows(x, lead, n)
+    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+    code = _lib.load().b200ait_quantize_rows(_ptr(q), _ptr(scale), _ptr(x), math.prod(lead), n, pitch, _padded(n),
+                                             UNARY[activation], int(gated), _dtype_code(x), _stream())
+    _lib.check(code, "b200ait_quantize_rows")
+    return q, scale
+
+
+def gemm_rcr_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale: Optional[torch.Tensor] = None,
+                bias: Optional[torch.Tensor] = None, d0: Optional[torch.Tensor] = None, d1: Optional[torch.Tensor] = None,
+                epilogue: str = "", dtype: Optional[torch.dtype] = None, tile_n: int = 0) -> torch.Tensor:
+    """y = epilogue((x @ w.T) * x_scale[:, None] * w_scale + bias, d0, d1) of signed 8-bit integers, in 16 bits.
+
+    w int8 [N, K] with w_scale fp32 [N]; x int8 [..., K] with x_scale fp32 [...], as quantize_rows makes them, or x in 16 bits and no
+    x_scale: its rows are then quantised on the way. Sums are exact (K up to 131071). The epilogues are gemm_rcr's. `dtype`: of
+    y, bias, d0 and d1 (default: x's if that has 16 bits, else d0's or the bias's, else float16). Rows of x and w may lie apart;
+    the tensor cores want them to start on 16 bytes (a pitch that is a multiple of 16), other rows take a slower kernel."""
+    what = "gemm_rcr_i8"
+    _check_here(what, x=x, w=w, w_scale=w_scale, x_scale=x_scale, bias=bias, d0=d0, d1=d1)
+    if w.dim() != 2 or x.dim() < 1 or w.shape[1] != x.shape[-1]:
+        raise ValueError(f"{what}: K mismatch {tuple(x.shape)} vs {tuple(w.shape)}")
+    n, k = w.shape
+    if k == 0:
+        raise ValueError(f"{what}: K is 0")
+    if w.dtype != torch.int8:
+        raise ValueError(f"{what}: w must be int8, got {w.dtype}")
+    if dtype is None:
+        given = [t.dtype for t in (x, d0, bias) if t is not None and t.dtype != torch.int8]
+        dtype = given[0] if given else torch.float16
+    if dtype not in _DTYPE_CODE:
+        raise ValueError(f"unsupported dtype {dtype}: the kernels take float16 or bfloat16")
+    if x.dtype == torch.int8:
+        if x_scale is None:
+            raise ValueError(f"{what}: an int8 x needs x_scale")
+    elif x_scale is not None:
+        raise ValueError(f"{what}: x_scale goes with an int8 x, got {x.dtype}")
+    else:
+        x, x_scale = quantize_rows(x)
+    lead = x.shape[:-1]
+    for name, t, shape in (("w_scale", w_scale, (n,)), ("x_scale", x_scale, tuple(lead))):
+        if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous float32 tensor of shape {shape}")
+    if epilogue not in EPILOGUES:
+        raise ValueError(f"{what}: unknown epilogue {epilogue}")
+    _, b1, b2, _ = EPILOGUES[epilogue]
+    out_shape = (*lead, n)
+    for name, t, wanted, shape in (("bias", bias, bias is not None, (n,)), ("d0", d0, b1 is not None, out_shape),
+                                   ("d1", d1, b2 is not None, out_shape)):
+        if not wanted:
+            if t is not None:
+                raise ValueError(f"{what}: the epilogue '{epilogue}' takes no {name}")
+            continue
+        if t is None:
+            raise ValueError(f"{what}: the epilogue '{epilogue}' needs {name}")
+        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {shape}")
+    lda, ldb = _row_pitch(what, "x", x), _row_pitch(what, "w", w)
+    m = math.prod(lead)
+    y = torch.empty(out_shape, dtype=dtype, device=x.device)
+    code = _lib.load().b200ait_gemm_rcr_i8(_ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(bias), _ptr(d0), _ptr(d1), _ptr(y),
+                                           m, n, k, _padded(k) if m == 1 else lda, _padded(k) if n == 1 else ldb, n, n,
+                                           epilogue_code(epilogue), _DTYPE_CODE[dtype], tile_n, _stream())
+    _lib.check(code, "b200ait_gemm_rcr_i8")
+    return y
+
+
+NORMS = {None: 0, "layer": 1, "rms": 2}
+
+
+def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                  post_gamma: Optional[torch.Tensor] = None, post_beta: Optional[torch.Tensor] = None,
+                  gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None, post_norm: Optional[str] = None,
+                  norm: str = "layer", residual_scale: float = 1.0, eps: float = 1e-5, quantize: bool = False):
+    """What stands between two blocks of a transformer, in one pass over the rows of x [..., N]:
+        p = post_norm(x) * post_gamma + post_beta;  total = residual_scale * residual + gate * p;  y = norm(total) * gamma + beta
+    Returns (total, y), or with `quantize` (total, q, scale): y as int8 rows with a scale each, as quantize_rows makes them.
+
+    norm and post_norm: "layer" or "rms", post_norm None for no norm after the block. residual, gate, the gammas and the betas may be
+    left out. post_gamma and post_beta are [N]; gate, gamma and beta [N] or [G, N], a vector for each of G equal parts of the rows
+    (a gate per sample). y comes of the unrounded total."""
+    what = "residual_norm"
+    operands = dict(x=x, residual=residual, gate=gate, post_gamma=post_gamma, post_beta=post_beta, gamma=gamma, beta=beta)
+    _check_here(what, **operands)
+    if norm not in ("layer", "rms") or post_norm not in NORMS:
+        raise ValueError(f"{what}: a norm is 'layer' or 'rms', got {norm!r} and {post_norm!r}")
+    if post_norm is None and (post_gamma is not None or post_beta is not None):
+        raise ValueError(f"{what}: post_gamma and post_beta need a post_norm")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{what}: x has no columns")
+    n, lead = x.shape[-1], x.shape[:-1]
+    rows = math.prod(lead)
+    parts = {}
+    for name, t in operands.items():
+        if t is None:
+            continue
+        if t.dtype != x.dtype or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous {x.dtype} tensor")
+        if name in ("x", "residual"):
+            fits = t.shape == x.shape
+        elif name in ("post_gamma", "post_beta"):
+            fits = tuple(t.shape) == (n,)
+        else:
+            parts[name] = t.shape[0] if t.dim() == 2 else 1
+            fits = t.dim() in (1, 2) and t.shape[-1] == n and parts[name] > 0 and rows % parts[name] == 0
+        if not fits:
+            raise ValueError(f"{what}: {name} of shape {tuple(t.shape)} does not fit x of shape {tuple(x.shape)}")
+    total = torch.empty_like(x)
+    if quantize:
+        y, scale = _int8_rows(x, lead, n), torch.empty(lead, dtype=torch.float32, device=x.device)
+    else:
+        y, scale = torch.empty_like(x), None
+    code = _lib.load().b200ait_residual_norm(
+        _ptr(total), _ptr(y), _ptr(scale), _ptr(x), _ptr(residual), _ptr(gate), _ptr(post_gamma), _ptr(post_beta), _ptr(gamma),
+        _ptr(beta), rows, n, parts.get("gate", 1), parts.get("gamma", 1), parts.get("beta", 1), _padded(n), NORMS[post_norm],
+        NORMS[norm], residual_scale, eps, _dtype_code(x), _stream())
+    _lib.check(code, "b200ait_residual_norm")
+    return (total, y, scale) if quantize else (total, y)
+
+
 def layernorm(x: torch.Tensor, gamma: Optional[torch.Tensor], beta: Optional[torch.Tensor], eps: float = 1e-5,
               normalized_ndim: int = 1) -> torch.Tensor:
     y = (_calls or _native()).layernorm(x, gamma, beta, eps, normalized_ndim)

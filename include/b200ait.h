@@ -124,6 +124,17 @@ int b200ait_gemm_rcr_static_scratch(const void* a, const void* b, const void* bi
                                     int epilogue, int dtype, float alpha, int store_mode, int64_t t1, int64_t t2,
                                     int64_t t3, int tile_n, int split_k, int* status_out, b200ait_stream_t stream);
 
+/* gemm_rcr of signed 8-bit integers with a scale per row of either operand:
+ *   c[m, n] = epilogue(sum_k a[m, k] b[n, k] * b_scale[n] * a_scale[m] + bias[n], d0, d1)
+ * a [m, k] (row pitch lda), b [n, k] (row pitch ldb), both int8; the scales are fp32 device vectors; bias, d0, d1 and c have the 16-bit
+ * type `dtype`. Sums are exact 32-bit integers (k <= 131071), scaled and run through the epilogue in fp32, rounded once. Operands
+ * that start on 16 bytes with pitches of whole 16 bytes go to the tensor cores whatever k is; others take a slower kernel.
+ * tile_n as for b200ait_gemm_rcr. A scale that is NaN (b200ait_quantize_rows) makes its row NaN. No counterpart in the reference,
+ * whose GEMMs take 16- and 32-bit floats only. */
+int b200ait_gemm_rcr_i8(const void* a, const float* a_scale, const void* b, const float* b_scale, const void* bias,
+                        const void* d0, const void* d1, void* c, int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb,
+                        int64_t ldc, int64_t ldd, int epilogue, int dtype, int tile_n, b200ait_stream_t stream);
+
 /* fp16 entry points with the reference's generated signatures. workspace / split_k are accepted
  * and ignored. *c_dim0, *c_dim1 are written.
  * gemm_rcr: python/aitemplate/backend/cuda/gemm_universal/common.py:172-198 */
@@ -212,6 +223,24 @@ int b200ait_flash_attention(void* output, const void* qkv, const int* cu_seqlens
 int b200ait_layernorm(void* out, const void* in, const void* gamma, const void* beta, int64_t m, int64_t n,
                       float eps, int64_t in_row_stride, int64_t out_row_stride, int dtype,
                       b200ait_stream_t stream);
+
+/* Rows of 16-bit values to signed 8-bit ones with a scale each: q = round(127 v / max |v|) to the nearest, ties to even, and scale =
+ * max |v| / 127, with v = act(x[:, :n]), or with `gated` act(x[:, :n]) * x[:, n:2n]. A row of zeros has scale 0 and q 0, a row with
+ * an infinity or a NaN scale NaN and q 0. Row pitches in elements; bytes of q between n and its pitch are left alone. `activation`:
+ * one of B200AIT_UNARY_*. No counterpart in the reference. */
+int b200ait_quantize_rows(void* q, float* scale, const void* x, int64_t rows, int64_t n, int64_t x_pitch, int64_t q_pitch,
+                          int activation, int gated, int dtype, b200ait_stream_t stream);
+
+/* What stands between two blocks of a transformer, in one pass over [rows, n]:
+ *   p = post_norm(x) * post_gamma + post_beta;  sum = residual_scale * residual + gate * p;  y = norm(sum) * gamma + beta
+ * post_norm: 0 none (p = x), 1 layer, 2 rms; norm: 1 layer, 2 rms. residual, gate, the gammas, the betas and the output `sum` may be NULL
+ * (left out). gate, gamma and beta hold `gates`, `gammas`, `betas` vectors of n, one for each of as many equal parts of the rows. y has the
+ * inputs' type (rows of n), or with y_scale not NULL signed 8-bit integers (row pitch y_pitch) with a scale per row as by
+ * b200ait_quantize_rows. `sum` may be `residual` or `x`. Next of kin in the reference: layernorm_sigmoid_mul.py:72-83. */
+int b200ait_residual_norm(void* sum, void* y, float* y_scale, const void* x, const void* residual, const void* gate,
+                          const void* post_gamma, const void* post_beta, const void* gamma, const void* beta, int64_t rows,
+                          int64_t n, int64_t gates, int64_t gammas, int64_t betas, int64_t y_pitch, int post_norm, int norm,
+                          float residual_scale, float eps, int dtype, b200ait_stream_t stream);
 
 /* softmax over the middle axis of a tensor viewed as [outer, k, inner]
  * (python/aitemplate/backend/cuda/softmax/softmax.py:142-153) */
