@@ -17,10 +17,11 @@ struct QuantizeParams {
   int n, activation;
 };
 
-template <int VEC, int CNT, bool BLOCK, bool GATED, bool BF16>
-__global__ void __launch_bounds__(BLOCK ? kTeamMaxThreads : 32 * kTeamWarpsPerBlock) quantize_rows_kernel(const QuantizeParams p) {
+template <int VEC, int CNT, int MOST, bool GATED, bool BF16>
+__global__ void __launch_bounds__(kTeamBlock<MOST>) quantize_rows_kernel(const QuantizeParams p) {
   grid_release();
   grid_wait();
+  constexpr bool BLOCK = MOST > 32;
   using T = typename Elem16<BF16>::T;
   using Raw = RawUnit<VEC>;
   __shared__ uint32_t words[1][32];
@@ -90,12 +91,13 @@ __global__ void __launch_bounds__(kTeamMaxThreads) quantize_long_rows_kernel(con
   }
 }
 
-template <int VEC, int CNT, bool BLOCK, bool GATED, bool BF16>
+template <int VEC, int CNT, int MOST, bool GATED, bool BF16>
 static void launch_quantize(const QuantizeParams& p, int threads, cudaStream_t stream) {
+  constexpr bool BLOCK = MOST > 32;
   const long long blocks = BLOCK ? p.rows : (p.rows + kTeamWarpsPerBlock - 1) / kTeamWarpsPerBlock;
   const int block = BLOCK ? threads : 32 * kTeamWarpsPerBlock;
   const bool early = blocks_start_early(blocks, block, sm_count(), 2048) || !in_capture(stream);
-  launch_early(&quantize_rows_kernel<VEC, CNT, BLOCK, GATED, BF16>, dim3(static_cast<unsigned>(blocks)), block, 0, stream, early, 1, p);
+  launch_early(&quantize_rows_kernel<VEC, CNT, MOST, GATED, BF16>, dim3(static_cast<unsigned>(blocks)), block, 0, stream, early, 1, p);
 }
 
 template <bool GATED, bool BF16>
@@ -107,22 +109,9 @@ static void quantize_dispatch(const QuantizeParams& p, bool vector_ok, cudaStrea
     B200AIT_CUDA_CHECK(cudaGetLastError());
     return;
   }
-  switch ((t.vec == 1 ? 100 : t.block ? 10 : 0) + t.cnt) {
-#define B200AIT_CASE(AT, VEC, CNT, BLOCK) \
-  case (AT) + (CNT): return launch_quantize<VEC, CNT, BLOCK, GATED, BF16>(p, t.threads, stream);
-    B200AIT_CASE(0, 8, 1, false)
-    B200AIT_CASE(0, 8, 2, false)
-    B200AIT_CASE(0, 8, 3, false)
-    B200AIT_CASE(0, 8, 4, false)
-    B200AIT_CASE(10, 8, 1, true)
-    B200AIT_CASE(10, 8, 2, true)
-    B200AIT_CASE(10, 8, 3, true)
-    B200AIT_CASE(10, 8, 4, true)
-    B200AIT_CASE(100, 1, 8, true)
-    B200AIT_CASE(100, 1, 32, true)
-#undef B200AIT_CASE
-  }
-  throw Error("quantize_rows: no kernel for this row");
+  for_team_shape(t, [&](auto vec, auto cnt, auto most) {
+    launch_quantize<decltype(vec)::value, decltype(cnt)::value, decltype(most)::value, GATED, BF16>(p, t.threads, stream);
+  });
 }
 
 }  // namespace b200ait

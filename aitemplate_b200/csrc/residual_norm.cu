@@ -52,11 +52,12 @@ __device__ __forceinline__ void normalize_row(const RowTeam<BLOCK>& team, float 
   for (int i = 0; i < CNT * VEC; ++i) v[i] = (v[i] - mean) * rstd;
 }
 
-template <int VEC, int CNT, bool BLOCK, bool QUANTIZE, bool BF16>
-__global__ void __launch_bounds__(BLOCK ? kTeamMaxThreads : 32 * kTeamWarpsPerBlock)
+template <int VEC, int CNT, int MOST, bool QUANTIZE, bool BF16>
+__global__ void __launch_bounds__(kTeamBlock<MOST>)
     residual_norm_kernel(const ResidualNormParams p) {
   grid_release();
   grid_wait();
+  constexpr bool BLOCK = MOST > 32;
   using T = typename Elem16<BF16>::T;
   using Raw = RawUnit<VEC>;
   using Unit = typename Raw::Type;
@@ -204,12 +205,13 @@ __global__ void __launch_bounds__(kTeamMaxThreads) residual_norm_long_rows_kerne
   }
 }
 
-template <int VEC, int CNT, bool BLOCK, bool QUANTIZE, bool BF16>
+template <int VEC, int CNT, int MOST, bool QUANTIZE, bool BF16>
 static void launch_residual_norm(const ResidualNormParams& p, int threads, cudaStream_t stream) {
+  constexpr bool BLOCK = MOST > 32;
   const long long blocks = BLOCK ? p.rows : (p.rows + kTeamWarpsPerBlock - 1) / kTeamWarpsPerBlock;
   const int block = BLOCK ? threads : 32 * kTeamWarpsPerBlock;
   const bool early = blocks_start_early(blocks, block, sm_count(), 2048) || !in_capture(stream);
-  launch_early(&residual_norm_kernel<VEC, CNT, BLOCK, QUANTIZE, BF16>, dim3(static_cast<unsigned>(blocks)), block, 0, stream, early, 1,
+  launch_early(&residual_norm_kernel<VEC, CNT, MOST, QUANTIZE, BF16>, dim3(static_cast<unsigned>(blocks)), block, 0, stream, early, 1,
                p);
 }
 
@@ -222,22 +224,9 @@ static void residual_norm_dispatch(const ResidualNormParams& p, bool vector_ok, 
     B200AIT_CUDA_CHECK(cudaGetLastError());
     return;
   }
-  switch ((t.vec == 1 ? 100 : t.block ? 10 : 0) + t.cnt) {
-#define B200AIT_CASE(AT, VEC, CNT, BLOCK) \
-  case (AT) + (CNT): return launch_residual_norm<VEC, CNT, BLOCK, QUANTIZE, BF16>(p, t.threads, stream);
-    B200AIT_CASE(0, 8, 1, false)
-    B200AIT_CASE(0, 8, 2, false)
-    B200AIT_CASE(0, 8, 3, false)
-    B200AIT_CASE(0, 8, 4, false)
-    B200AIT_CASE(10, 8, 1, true)
-    B200AIT_CASE(10, 8, 2, true)
-    B200AIT_CASE(10, 8, 3, true)
-    B200AIT_CASE(10, 8, 4, true)
-    B200AIT_CASE(100, 1, 8, true)
-    B200AIT_CASE(100, 1, 32, true)
-#undef B200AIT_CASE
-  }
-  throw Error("residual_norm: no kernel for this row");
+  for_team_shape(t, [&](auto vec, auto cnt, auto most) {
+    launch_residual_norm<decltype(vec)::value, decltype(cnt)::value, decltype(most)::value, QUANTIZE, BF16>(p, t.threads, stream);
+  });
 }
 
 }  // namespace b200ait

@@ -3,6 +3,7 @@
 // signed 8-bit ones with a scale per row.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "epilogue.cuh"
@@ -13,6 +14,10 @@ namespace b200ait {
 
 constexpr int kTeamMaxThreads = 1024;
 constexpr int kTeamWarpsPerBlock = 8;  // rows of a block where a warp takes a row
+
+// threads of a block whose teams have up to MOST
+template <int MOST>
+constexpr int kTeamBlock = MOST == 32 ? 32 * kTeamWarpsPerBlock : MOST;
 
 // A reduction needs one barrier: each has words of its own (`slot`), so no thread can overwrite what another still reads.
 template <bool BLOCK>
@@ -152,25 +157,45 @@ __device__ __forceinline__ void store_quantized(int8_t* row, long long unit, con
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// How a row of n elements is laid over threads (rows too long for that are walked: team = 0).
+// How a row of n elements is laid over threads: `cnt` units of `vec` elements each (0: the row is too long and is walked), by a warp
+// (most = 32) or by a block of `threads` whose kernel is built for up to `most`.
 struct TeamShape {
-  int vec, cnt, threads;
-  bool block;
+  int vec, cnt, threads, most;
 };
 inline TeamShape team_shape(long long rows, long long n, bool vector_ok, int sms) {
-  const long long units = vector_ok ? n / 8 : n;
+  auto shape = [](int vec, long long units, long long per) {
+    const int t = static_cast<int>(std::max<long long>(32, ((units + per - 1) / per + 31) / 32 * 32));
+    const int cnt = static_cast<int>(std::max<long long>(1, (units + t - 1) / t));
+    return TeamShape{vec, cnt, t, t == 32 && vec == 8 ? 32 : t <= 256 ? 256 : t <= 512 ? 512 : 1024};
+  };
   if (!vector_ok) {
-    if (units > 32ll * kTeamMaxThreads) return TeamShape{1, 0, kTeamMaxThreads, true};
-    const int cnt = units <= 8ll * kTeamMaxThreads ? 8 : 32;
-    const long long t = std::max<long long>(32, ((units + cnt - 1) / cnt + 31) / 32 * 32);
-    return TeamShape{1, cnt, static_cast<int>(t), true};
+    if (n > 32ll * kTeamMaxThreads) return TeamShape{1, 0, kTeamMaxThreads, kTeamMaxThreads};
+    TeamShape t = shape(1, n, n <= 8ll * kTeamMaxThreads ? 8 : 32);
+    t.cnt = n <= 8ll * kTeamMaxThreads ? 8 : 32, t.most = kTeamMaxThreads;
+    return t;
   }
-  if (units > 4ll * kTeamMaxThreads) return TeamShape{8, 0, kTeamMaxThreads, true};
+  const long long units = n / 8;
+  if (units > 4ll * kTeamMaxThreads) return TeamShape{8, 0, kTeamMaxThreads, kTeamMaxThreads};
   // A few rows are a matter of latency: a unit a thread. Many are one of bytes in flight: up to four.
-  const long long per = rows <= 2ll * sms && units <= kTeamMaxThreads ? 1 : 4;
-  const long long t = std::max<long long>(32, ((units + per - 1) / per + 31) / 32 * 32);
-  const int cnt = static_cast<int>(std::max<long long>(1, (units + t - 1) / t));
-  return TeamShape{8, cnt, static_cast<int>(t), t > 32};
+  return shape(8, units, rows <= 2ll * sms && units <= kTeamMaxThreads ? 1 : 4);
+}
+
+// Calls `launch` with (VEC, CNT, MOST) as compile-time numbers. Of block-wide shapes with 16-byte units only these come about: one unit
+// a thread, or four, and three where a block has 64 or 96 threads.
+template <int N>
+using TeamInt = std::integral_constant<int, N>;
+template <class F>
+inline void for_team_shape(const TeamShape& t, F&& launch) {
+  switch (t.vec * 100000 + t.most * 10 + (t.vec == 8 ? t.cnt : t.cnt == 32 ? 1 : 0)) {
+#define B200AIT_TEAM(VEC, CNT, MOST) \
+  case (VEC) * 100000 + (MOST) * 10 + ((VEC) == 8 ? (CNT) : (CNT) == 32 ? 1 : 0): return launch(TeamInt<VEC>{}, TeamInt<CNT>{}, TeamInt<MOST>{});
+    B200AIT_TEAM(8, 1, 32) B200AIT_TEAM(8, 2, 32) B200AIT_TEAM(8, 3, 32) B200AIT_TEAM(8, 4, 32)
+    B200AIT_TEAM(8, 1, 256) B200AIT_TEAM(8, 3, 256) B200AIT_TEAM(8, 4, 256)
+    B200AIT_TEAM(8, 1, 512) B200AIT_TEAM(8, 4, 512) B200AIT_TEAM(8, 1, 1024) B200AIT_TEAM(8, 4, 1024)
+    B200AIT_TEAM(1, 8, 1024) B200AIT_TEAM(1, 32, 1024)
+#undef B200AIT_TEAM
+  }
+  throw Error("no kernel for rows of this length");
 }
 
 }  // namespace b200ait
