@@ -144,7 +144,8 @@ def load() -> ctypes.CDLL:
 # entry points that csrc/torch_calls.cpp calls, in the order of its Library structure
 _CALLED = ["b200ait_gemm_rcr", "b200ait_gemm_rrr", "b200ait_gemm_rcr_scratch_bytes", "b200ait_mem_eff_attention",
            "b200ait_flash_attention", "b200ait_layernorm", "b200ait_softmax", "b200ait_concatenate", "b200ait_split",
-           "b200ait_permute", "b200ait_last_error", "AITemplateModelContainerRun"]
+           "b200ait_permute", "b200ait_last_error", "AITemplateModelContainerRun", "b200ait_gemm_rcr_i8",
+           "b200ait_quantize_rows", "b200ait_residual_norm"]
 _calls = None
 
 

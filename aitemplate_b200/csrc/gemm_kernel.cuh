@@ -227,12 +227,12 @@ __device__ __forceinline__ void epilogue_chunk32(const GemmParams& p, float (&v)
 }
 
 // What follows the bias in the fused epilogue of one element, and its store: activation, residual(s), activation, one rounding.
-template <bool BF16>
+template <bool BF16, bool I8 = false>
 __device__ __forceinline__ void epilogue_scalar_rest(const GemmParams& p, float v, int b, int row, int col) {
   using E = Elem16<BF16>;
   using T = typename E::T;
   const int u1 = epi_u1(p.epilogue), b1 = epi_b1(p.epilogue), b2 = epi_b2(p.epilogue), u2 = epi_u2(p.epilogue);
-  v = apply_unary(u1, v);
+  v = apply_unary_of<I8>(u1, v);
   const long long di = static_cast<long long>(b) * p.d_bs + static_cast<long long>(row) * p.ldd + col;
   if (b1 != kBinaryNone) {
     const float f = E::to_float(static_cast<const T*>(p.d0)[di]);
@@ -242,7 +242,7 @@ __device__ __forceinline__ void epilogue_scalar_rest(const GemmParams& p, float 
     const float f = E::to_float(static_cast<const T*>(p.d1)[di]);
     v = (b2 == kBinaryAdd) ? v + f : v * f;
   }
-  v = apply_unary(u2, v);
+  v = apply_unary_of<I8>(u2, v);
   static_cast<T*>(p.out)[batch_offset(p, b) + row_offset(p, row) + col_offset(p, col)] = E::from_float(v);
 }
 // The fused epilogue on one fp32 accumulator: alpha, bias and the rest.
@@ -258,7 +258,7 @@ __device__ __forceinline__ void epilogue_scalar_store_i8(const GemmParams& p, fl
   const float rs = p.row_scale[row];
   const float v = p.bias ? __fmaf_rn(scaled, rs, Elem16<BF16>::to_float(static_cast<const typename Elem16<BF16>::T*>(p.bias)[col]))
                          : scaled * rs;
-  epilogue_scalar_rest<BF16>(p, v, 0, row, col);
+  epilogue_scalar_rest<BF16, true>(p, v, 0, row, col);
 }
 
 // EPI >= 0 fixes the epilogue code at compile time (straight-line code for the common epilogues);
@@ -270,14 +270,14 @@ __device__ __forceinline__ int epilogue_code_of(const GemmParams& p) {
 
 // Fused epilogue math of the tensor-core kernel for 32 consecutive columns of one row. `v` already
 // holds alpha * acc + bias. d0 is prefetched by the caller (d0v valid when the chunk is `full`).
-template <bool BF16, int EPI>
+template <bool BF16, int EPI, bool I8 = false>
 __device__ __forceinline__ void epilogue_math32(const GemmParams& p, float (&v)[32], const uint4 (&d0v)[4], int b,
                                                 int row, int col0, bool full, bool row_ok) {
   using E = Elem16<BF16>;
   using T = typename E::T;
   const int code = epilogue_code_of<EPI>(p);
   const int u1 = epi_u1(code), b1 = epi_b1(code), b2 = epi_b2(code), u2 = epi_u2(code);
-  apply_unary_vec(u1, v);
+  apply_unary_vec_of<I8>(u1, v);
   const long long d_base = static_cast<long long>(b) * p.d_bs + static_cast<long long>(row) * p.ldd + col0;
   if (b1 != kBinaryNone && row_ok) {
     if (full) {
@@ -320,7 +320,7 @@ __device__ __forceinline__ void epilogue_math32(const GemmParams& p, float (&v)[
         }
     }
   }
-  apply_unary_vec(u2, v);
+  apply_unary_vec_of<I8>(u2, v);
 }
 
 // Direct register -> global store of 32 consecutive columns of one row.
@@ -855,7 +855,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
             for (int u = 0; u < 4; ++u)
               d0c[u] = *reinterpret_cast<const uint4*>(row_base + ((((c & 1) * 4 + u) ^ (lane & 7)) * 16));
           }
-          epilogue_math32<BF16, EPI>(p, v, d0c, b, row, col0, full || box_d0, row_ok);
+          epilogue_math32<BF16, EPI, I8>(p, v, d0c, b, row, col0, full || box_d0, row_ok);
           if (!box_d0 && (c & 1) == 0) {  // the box buffer is about to be rewritten: its last store must have read it
             if (lead) bulk_wait_group_read0();
             __syncwarp();
@@ -904,7 +904,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
             for (int u = 0; u < 4; ++u)
               d0c[u] = *reinterpret_cast<const uint4*>(row_base + ((((c & 1) * 4 + u) ^ (lane & 7)) * 16));
           }
-          epilogue_math32<BF16, EPI>(p, v, d0c, b, row, col0, full || row_d0, row_ok);
+          epilogue_math32<BF16, EPI, I8>(p, v, d0c, b, row, col0, full || row_d0, row_ok);
 #pragma unroll
           for (int u = 0; u < 4; ++u)
             *reinterpret_cast<uint4*>(row_base + ((((c & 1) * 4 + u) ^ (lane & 7)) * 16)) = pack8<BF16>(&v[u * 8]);
@@ -914,7 +914,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
             __syncwarp();
           }
         } else if (row_ok) {
-          epilogue_math32<BF16, EPI>(p, v, d0c, b, row, col0, full, true);
+          epilogue_math32<BF16, EPI, I8>(p, v, d0c, b, row, col0, full, true);
           epilogue_direct_store32<BF16>(p, v, b, row, col0, full, chunk_contig);
         }
       };

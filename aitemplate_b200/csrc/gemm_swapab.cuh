@@ -370,7 +370,7 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_const
             float w[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = w[e] * factor + bias_v[e];
-            apply_unary_vec(u1, w);
+            apply_unary_vec_of<I8>(u1, w);
             *reinterpret_cast<float4*>(src) = make_float4(w[0], w[1], w[2], w[3]);
             *reinterpret_cast<float4*>(src + 4) = make_float4(w[4], w[5], w[6], w[7]);
           }
@@ -460,7 +460,7 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_const
                 for (int e = 0; e < 8; ++e) o[t * 8 + e] = (b2 == kBinaryAdd) ? o[t * 8 + e] + f[e] : o[t * 8 + e] * f[e];
               }
             }
-            apply_unary_vec(u2, o);
+            apply_unary_vec_of<I8>(u2, o);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
               if (j + 8 * t < my_rows)

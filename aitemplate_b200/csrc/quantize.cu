@@ -17,100 +17,92 @@ struct QuantizeParams {
   int n, activation;
 };
 
-template <int VEC, int CNT, int MOST, bool GATED, bool BF16>
-__global__ void __launch_bounds__(kTeamBlock<MOST>) quantize_rows_kernel(const QuantizeParams p) {
+template <int CNT, int THREADS, bool ALIGNED, bool GATED, bool BF16>
+__global__ void __launch_bounds__(kTeamBlock<THREADS>) quantize_rows_kernel(const QuantizeParams p) {
   grid_release();
   grid_wait();
-  constexpr bool BLOCK = MOST > 32;
-  using T = typename Elem16<BF16>::T;
-  using Raw = RawUnit<VEC>;
+  using Team = RowTeam<CNT, THREADS, ALIGNED>;
   __shared__ uint32_t words[1][32];
-  const RowTeam<BLOCK> team{words, BLOCK ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x & 31),
-                            BLOCK ? static_cast<int>(blockDim.x) : 32};
-  const long long row = BLOCK ? static_cast<long long>(blockIdx.x)
-                              : static_cast<long long>(blockIdx.x) * kTeamWarpsPerBlock + (threadIdx.x >> 5);
+  __shared__ uint2 staged[kTeamBlock<THREADS> / THREADS][Team::kStagedBytes / 8];
+  const long long row = Team::row();
   if (row >= p.rows) return;
-  const int units = p.n / VEC;
-  const T* x = static_cast<const T*>(p.x) + row * p.x_pitch;
-  typename Raw::Type raw[CNT], up[GATED ? CNT : 1];
+  const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.x_pitch;
+  const uint16_t* lo = static_cast<const uint16_t*>(p.x);
+  const uint16_t* hi = lo + (p.rows - 1) * p.x_pitch + (GATED ? 2 * p.n : p.n);
+  const Team team(words, p.n, x);
+  uint4 raw[CNT], up[GATED ? CNT : 1];
 #pragma unroll
   for (int i = 0; i < CNT; ++i) {
-    const int u = team.tid + i * team.threads;
-    raw[i] = u < units ? ld_stream(reinterpret_cast<const typename Raw::Type*>(x) + u) : Raw::zero();
-    if (GATED) up[i] = u < units ? ld_stream(reinterpret_cast<const typename Raw::Type*>(x + p.n) + u) : Raw::zero();
+    raw[i] = team.template load<true>(x, lo, hi, i);
+    if (GATED) up[i] = ALIGNED ? team.template load<true>(x + p.n, lo, hi, i) : team.load_off(x + p.n, lo, hi, i);
   }
-  float v[CNT * VEC];
+  float v[CNT * 8];
 #pragma unroll
-  for (int i = 0; i < CNT; ++i) unpack_unit<VEC, BF16>(raw[i], &v[i * VEC]);
-  if (p.activation != kUnaryIdentity) apply_unary_vec(p.activation, v);
+  for (int i = 0; i < CNT; ++i) unpack8<BF16>(raw[i], &v[i * 8]);
+  if (p.activation != kUnaryIdentity) apply_unary_vec_of<true>(p.activation, v);
   uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < CNT; ++i) {
     if (GATED) {
-      float f[VEC];
-      unpack_unit<VEC, BF16>(up[i], f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i * VEC + j] *= f[j];
+      float f[8];
+      unpack8<BF16>(up[i], f);
+      by_pairs<8>(&v[i * 8], [&](uint64_t a, int j) { return mul2(a, pack2(f[j], f[j + 1])); });
     }
-    if (team.tid + i * team.threads < units) {  // (an activation of the zeros past the end need not be 0)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) most = max(most, magnitude_bits(v[i * VEC + j]));
-    }
+    team.clear_rest(&v[i * 8], i);
+    take_magnitudes<8>(most, &v[i * 8]);
   }
   const RowScale s = row_scale_of(team.most(most, 0));
   if (team.tid == 0) p.scale[row] = s.scale;
-  int8_t* q = p.q + row * p.q_pitch;
+  uint2 b[CNT];
 #pragma unroll
-  for (int i = 0; i < CNT; ++i) {
-    const int u = team.tid + i * team.threads;
-    if (u < units) store_quantized<VEC>(q, u, s, &v[i * VEC]);
-  }
+  for (int i = 0; i < CNT; ++i) b[i] = quantize_unit(s, &v[i * 8]);
+  team.store_bytes(p.q + row * p.q_pitch, b, staged[threadIdx.x / THREADS]);
 }
 
-// Rows longer than the registers of a block hold (32768 elements): a block walks its row twice, the second time out of L2.
+// Rows longer than the registers of a block hold (32768 elements), or results at an odd place: a block walks its row twice, the
+// second time out of L2.
 template <bool BF16>
 __global__ void __launch_bounds__(kTeamMaxThreads) quantize_long_rows_kernel(const QuantizeParams p, const bool gated) {
   using E = Elem16<BF16>;
   using T = typename E::T;
   __shared__ uint32_t words[1][32];
-  const RowTeam<true> team{words, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
+  const RowTeam<1, kTeamMaxThreads, true> team(words, p.n, nullptr);
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.x_pitch;
   auto value = [&](int i) {
-    const float v = apply_unary(p.activation, E::to_float(x[i]));
+    const float v = apply_unary_of<true>(p.activation, E::to_float(x[i]));
     return gated ? v * E::to_float(x[p.n + i]) : v;
   };
   uint32_t most = 0;
-  for (int i = team.tid; i < p.n; i += team.threads) most = max(most, magnitude_bits(value(i)));
+  for (int i = team.tid; i < p.n; i += kTeamMaxThreads) {
+    const float v = value(i);
+    take_magnitudes<1>(most, &v);
+  }
   const RowScale s = row_scale_of(team.most(most, 0));
   if (team.tid == 0) p.scale[row] = s.scale;
   int8_t* q = p.q + row * p.q_pitch;
-  for (int i = team.tid; i < p.n; i += team.threads) {
-    const float v = value(i);
-    store_quantized<1>(q, i, s, &v);
-  }
+  for (int i = team.tid; i < p.n; i += kTeamMaxThreads) q[i] = quantize_value(s, value(i));
 }
 
-template <int VEC, int CNT, int MOST, bool GATED, bool BF16>
-static void launch_quantize(const QuantizeParams& p, int threads, cudaStream_t stream) {
-  constexpr bool BLOCK = MOST > 32;
-  const long long blocks = BLOCK ? p.rows : (p.rows + kTeamWarpsPerBlock - 1) / kTeamWarpsPerBlock;
-  const int block = BLOCK ? threads : 32 * kTeamWarpsPerBlock;
-  const bool early = blocks_start_early(blocks, block, sm_count(), 2048) || !in_capture(stream);
-  launch_early(&quantize_rows_kernel<VEC, CNT, MOST, GATED, BF16>, dim3(static_cast<unsigned>(blocks)), block, 0, stream, early, 1, p);
+template <int CNT, int THREADS, bool ALIGNED, bool GATED, bool BF16>
+static void launch_quantize(const QuantizeParams& p, cudaStream_t stream) {
+  constexpr int kBlock = kTeamBlock<THREADS>;
+  const long long blocks = THREADS > 32 ? p.rows : (p.rows + kTeamWarpsPerBlock - 1) / kTeamWarpsPerBlock;
+  const bool early = blocks_start_early(blocks, kBlock, sm_count(), 2048) || !in_capture(stream);
+  launch_early(&quantize_rows_kernel<CNT, THREADS, ALIGNED, GATED, BF16>, dim3(static_cast<unsigned>(blocks)), kBlock, 0, stream, early, 1, p);
 }
 
 template <bool GATED, bool BF16>
-static void quantize_dispatch(const QuantizeParams& p, bool vector_ok, cudaStream_t stream) {
-  const TeamShape t = team_shape(p.rows, p.n, vector_ok, sm_count());
-  if (t.cnt == 0) {
+static void quantize_dispatch(const QuantizeParams& p, bool lie_well, bool aligned, cudaStream_t stream) {
+  const TeamShape t = team_shape(p.rows, p.n, aligned, sm_count());
+  if (t.cnt == 0 || !lie_well) {
     count_launch();
-    quantize_long_rows_kernel<BF16><<<static_cast<unsigned>(p.rows), t.threads, 0, stream>>>(p, GATED);
+    quantize_long_rows_kernel<BF16><<<static_cast<unsigned>(p.rows), kTeamMaxThreads, 0, stream>>>(p, GATED);
     B200AIT_CUDA_CHECK(cudaGetLastError());
     return;
   }
-  for_team_shape(t, [&](auto vec, auto cnt, auto most) {
-    launch_quantize<decltype(vec)::value, decltype(cnt)::value, decltype(most)::value, GATED, BF16>(p, t.threads, stream);
+  for_team_shape(t, [&](auto cnt, auto threads, auto whole) {
+    launch_quantize<decltype(cnt)::value, decltype(threads)::value, decltype(whole)::value, GATED, BF16>(p, stream);
   });
 }
 
@@ -128,17 +120,18 @@ B200AIT_EXPORT int b200ait_quantize_rows(void* q, float* scale, const void* x, i
     B200AIT_REQUIRE(q && scale && x, "quantize_rows: null pointer with non-zero size");
     B200AIT_REQUIRE(rows < (1ll << 31) && n < (1ll << 30), "quantize_rows: dimension exceeds int32");
     B200AIT_REQUIRE(x_pitch >= (gated ? 2 * n : n) && q_pitch >= n, "quantize_rows: a row pitch is shorter than the row");
-    auto aligned = [](const void* ptr, unsigned to) { return (reinterpret_cast<uintptr_t>(ptr) & (to - 1)) == 0; };
-    const bool vector_ok = n % 8 == 0 && x_pitch % 8 == 0 && q_pitch % 8 == 0 && aligned(x, 16) && aligned(q, 8);
+    B200AIT_REQUIRE(multiple_of(x, 2) && multiple_of(scale, 4), "quantize_rows: a pointer is not aligned to its type");
+    const bool lie_well = multiple_of(q, 8) && q_pitch % 8 == 0;
+    const bool aligned = n % 8 == 0 && x_pitch % 8 == 0 && multiple_of(x, 16);
     const QuantizeParams p{x, static_cast<int8_t*>(q), scale, rows, x_pitch, q_pitch, static_cast<int>(n), activation};
     const bool bf16 = dtype == kDTypeBFloat16;
     if (gated && bf16)
-      quantize_dispatch<true, true>(p, vector_ok, stream);
+      quantize_dispatch<true, true>(p, lie_well, aligned, stream);
     else if (gated)
-      quantize_dispatch<true, false>(p, vector_ok, stream);
+      quantize_dispatch<true, false>(p, lie_well, aligned, stream);
     else if (bf16)
-      quantize_dispatch<false, true>(p, vector_ok, stream);
+      quantize_dispatch<false, true>(p, lie_well, aligned, stream);
     else
-      quantize_dispatch<false, false>(p, vector_ok, stream);
+      quantize_dispatch<false, false>(p, lie_well, aligned, stream);
   });
 }

@@ -25,132 +25,122 @@ struct ResidualNormParams {
   float residual_scale, eps;
 };
 
-// normalises the row in `v`: layer or rms, without gamma and beta. `slot` and slot + 1 are the reductions' words.
-template <int VEC, int CNT, bool BLOCK>
-__device__ __forceinline__ void normalize_row(const RowTeam<BLOCK>& team, float (&v)[CNT * VEC], int kind, int units, float inv_n,
+// Turns the row in `v` into its norm, without gamma and beta. `slot` and slot + 1 are the reductions' words. What is not the row's
+// is 0 before and after.
+template <int CNT, int THREADS, bool ALIGNED>
+__device__ __forceinline__ void normalize_row(const RowTeam<CNT, THREADS, ALIGNED>& team, float (&v)[CNT * 8], int kind, float inv_n,
                                               float eps, int slot) {
-  float mean = 0.f;
+  float lo, hi;
   if (kind == kNormLayer) {
-    float s = 0.f;
+    uint64_t s = pack2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < CNT * VEC; ++i) s += v[i];  // (past the end of the row are zeros)
-    mean = team.sum(s, slot) * inv_n;
+    for (int j = 0; j < CNT * 8; j += 2) s = add2(s, pack2(v[j], v[j + 1]));
+    unpack2(s, lo, hi);
+    const float less = -team.sum(lo + hi, slot) * inv_n;
+    by_pairs<CNT * 8>(v, [&](uint64_t x, int) { return add2(x, pack2(less, less)); });
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) team.clear_rest(&v[i * 8], i);
   }
-  float q = 0.f;
+  uint64_t q = pack2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < CNT; ++i) {
-    if (team.tid + i * team.threads < units) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = v[i * VEC + j] - mean;
-        q = fmaf(d, d, q);
-      }
-    }
+  for (int j = 0; j < CNT * 8; j += 2) {
+    const uint64_t x = pack2(v[j], v[j + 1]);
+    q = fma2(x, x, q);
   }
-  const float rstd = rsqrtf(fmaf(team.sum(q, slot + 1), inv_n, eps));
-#pragma unroll
-  for (int i = 0; i < CNT * VEC; ++i) v[i] = (v[i] - mean) * rstd;
+  unpack2(q, lo, hi);
+  const float rstd = rsqrtf(fmaf(team.sum(lo + hi, slot + 1), inv_n, eps));
+  by_pairs<CNT * 8>(v, [&](uint64_t x, int) { return mul2(x, pack2(rstd, rstd)); });
 }
 
-template <int VEC, int CNT, int MOST, bool QUANTIZE, bool BF16>
-__global__ void __launch_bounds__(kTeamBlock<MOST>)
-    residual_norm_kernel(const ResidualNormParams p) {
+template <int CNT, int THREADS, bool ALIGNED, bool QUANTIZE, bool BF16>
+__global__ void __launch_bounds__(kTeamBlock<THREADS>) residual_norm_kernel(const ResidualNormParams p) {
   grid_release();
   grid_wait();
-  constexpr bool BLOCK = MOST > 32;
-  using T = typename Elem16<BF16>::T;
-  using Raw = RawUnit<VEC>;
-  using Unit = typename Raw::Type;
+  using Team = RowTeam<CNT, THREADS, ALIGNED>;
   __shared__ uint32_t words[5][32];
-  const RowTeam<BLOCK> team{words, BLOCK ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x & 31),
-                            BLOCK ? static_cast<int>(blockDim.x) : 32};
-  const long long row = BLOCK ? static_cast<long long>(blockIdx.x)
-                              : static_cast<long long>(blockIdx.x) * kTeamWarpsPerBlock + (threadIdx.x >> 5);
+  __shared__ uint2 staged[kTeamBlock<THREADS> / THREADS][QUANTIZE ? Team::kStagedBytes / 8 : 1];
+  const long long row = Team::row();
   if (row >= p.rows) return;
-  const int units = p.n / VEC;
+  const long long at = row * p.n, all = p.rows * p.n;
+  const Team team(words, p.n, static_cast<const uint16_t*>(p.x) + at);
   const float inv_n = 1.f / static_cast<float>(p.n);
-  auto unit_at = [&](int i) { return team.tid + i * team.threads; };
-  auto row_of = [&](const void* base, long long r) { return reinterpret_cast<const Unit*>(static_cast<const T*>(base) + r * p.n); };
-  Unit xr[CNT], rr[CNT];
+  uint4 xr[CNT], rr[CNT];
+  auto fetch = [&](const void* tensor, uint4 (&raw)[CNT]) {
+    const uint16_t* t = static_cast<const uint16_t*>(tensor);
 #pragma unroll
-  for (int i = 0; i < CNT; ++i) {
-    const int u = unit_at(i);
-    xr[i] = u < units ? ld_stream(row_of(p.x, row) + u) : Raw::zero();
-    rr[i] = p.residual != nullptr && u < units ? ld_stream(row_of(p.residual, row) + u) : Raw::zero();
-  }
-  float v[CNT * VEC];
+    for (int i = 0; i < CNT; ++i) raw[i] = team.template load<true>(t + at, t, t + all, i);
+  };
+  fetch(p.x, xr);
+  if (p.residual != nullptr) fetch(p.residual, rr);
+  float v[CNT * 8];
+  auto clear_rest = [&] {
 #pragma unroll
-  for (int i = 0; i < CNT; ++i) unpack_unit<VEC, BF16>(xr[i], &v[i * VEC]);
-  // v *= a or v += a, for a vector that rows share
-  auto times = [&](const void* base, long long r) {
-    const Unit* a = row_of(base, r);
+    for (int i = 0; i < CNT; ++i) team.clear_rest(&v[i * 8], i);
+  };
+#pragma unroll
+  for (int i = 0; i < CNT; ++i) unpack8<BF16>(xr[i], &v[i * 8]);
+  // every pair of values with the same two of vector r of those that `part` rows share each
+  auto with = [&](const void* vectors, long long r, long long part, auto&& f) {
+    const uint16_t* t = static_cast<const uint16_t*>(vectors);
+    const uint16_t* vector = t + r * p.n;
+    const uint16_t* end = t + (p.rows / part) * p.n;
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
-      float f[VEC];
-      unpack_unit<VEC, BF16>(unit_at(i) < units ? a[unit_at(i)] : Raw::zero(), f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i * VEC + j] *= f[j];
+      float a[8];
+      unpack8<BF16>(team.load_off(vector, t, end, i), a);
+      by_pairs<8>(&v[i * 8], [&](uint64_t x, int j) { return f(x, pack2(a[j], a[j + 1])); });
     }
   };
-  auto plus = [&](const void* base, long long r) {
-    const Unit* a = row_of(base, r);
-#pragma unroll
-    for (int i = 0; i < CNT; ++i) {
-      float f[VEC];
-      unpack_unit<VEC, BF16>(unit_at(i) < units ? a[unit_at(i)] : Raw::zero(), f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i * VEC + j] += f[j];
-    }
-  };
+  auto times = [](uint64_t x, uint64_t a) { return mul2(x, a); };
+  auto plus = [](uint64_t x, uint64_t a) { return add2(x, a); };
   if (p.post != kNormNone) {
-    normalize_row<VEC, CNT, BLOCK>(team, v, p.post, units, inv_n, p.eps, 0);
-    if (p.post_gamma) times(p.post_gamma, 0);
-    if (p.post_beta) plus(p.post_beta, 0);
+    clear_rest();
+    normalize_row(team, v, p.post, inv_n, p.eps, 0);
+    if (p.post_gamma) with(p.post_gamma, 0, p.rows, times);
+    if (p.post_beta) with(p.post_beta, 0, p.rows, plus);
   }
-  if (p.gate) times(p.gate, row / p.gate_part);
-#pragma unroll
-  for (int i = 0; i < CNT; ++i) {
-    float f[VEC];
-    unpack_unit<VEC, BF16>(rr[i], f);
-    const bool inside = unit_at(i) < units;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[i * VEC + j] = inside ? fmaf(p.residual_scale, f[j], v[i * VEC + j]) : 0.f;
-    if (p.sum != nullptr && inside)
-      store_unit<VEC, BF16>(static_cast<T*>(p.sum) + row * p.n, unit_at(i), &v[i * VEC]);
-  }
-  normalize_row<VEC, CNT, BLOCK>(team, v, p.norm, units, inv_n, p.eps, 2);
-  if (p.gamma) times(p.gamma, row / p.gamma_part);
-  if (p.beta) plus(p.beta, row / p.beta_part);
-  if constexpr (QUANTIZE) {
-    uint32_t most = 0;
+  if (p.gate) with(p.gate, row / p.gate_part, p.gate_part, times);
+  if (p.residual != nullptr) {
+    const uint64_t scale = pack2(p.residual_scale, p.residual_scale);
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
-      if (unit_at(i) < units) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) most = max(most, magnitude_bits(v[i * VEC + j]));
-      }
+      float r[8];
+      unpack8<BF16>(rr[i], r);
+      by_pairs<8>(&v[i * 8], [&](uint64_t a, int j) { return fma2(pack2(r[j], r[j + 1]), scale, a); });
     }
+  }
+  if (p.sum != nullptr) {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) team.template store<BF16>(static_cast<uint16_t*>(p.sum) + at, i, &v[i * 8]);
+  }
+  clear_rest();
+  normalize_row(team, v, p.norm, inv_n, p.eps, 2);
+  if (p.gamma) with(p.gamma, row / p.gamma_part, p.gamma_part, times);
+  if (p.beta) with(p.beta, row / p.beta_part, p.beta_part, plus);
+  if constexpr (QUANTIZE) {
+    clear_rest();
+    uint32_t most = 0;
+    take_magnitudes<CNT * 8>(most, v);
     const RowScale s = row_scale_of(team.most(most, 4));
     if (team.tid == 0) p.scale[row] = s.scale;
-    int8_t* q = static_cast<int8_t*>(p.y) + row * p.y_pitch;
+    uint2 b[CNT];
 #pragma unroll
-    for (int i = 0; i < CNT; ++i)
-      if (unit_at(i) < units) store_quantized<VEC>(q, unit_at(i), s, &v[i * VEC]);
+    for (int i = 0; i < CNT; ++i) b[i] = quantize_unit(s, &v[i * 8]);
+    team.store_bytes(static_cast<int8_t*>(p.y) + row * p.y_pitch, b, staged[threadIdx.x / THREADS]);
   } else {
 #pragma unroll
-    for (int i = 0; i < CNT; ++i)
-      if (unit_at(i) < units) store_unit<VEC, BF16>(static_cast<T*>(p.y) + row * p.n, unit_at(i), &v[i * VEC]);
+    for (int i = 0; i < CNT; ++i) team.template store<BF16>(static_cast<uint16_t*>(p.y) + at, i, &v[i * 8]);
   }
 }
 
-// Rows longer than the registers of a block hold: a block walks its row once for each statistic and once to write, after the first
+// Rows longer than the registers of a block hold, or operands that do not lie alike: a block walks its row once for each statistic and once to write, after the first
 // time out of L2, and works the sum out anew each time.
 template <bool QUANTIZE, bool BF16>
 __global__ void __launch_bounds__(kTeamMaxThreads) residual_norm_long_rows_kernel(const ResidualNormParams p) {
   using E = Elem16<BF16>;
   using T = typename E::T;
   __shared__ uint32_t words[5][32];
-  const RowTeam<true> team{words, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
+  const RowTeam<1, kTeamMaxThreads, true> team(words, p.n, nullptr);
   const long long row = blockIdx.x;
   const float inv_n = 1.f / static_cast<float>(p.n);
   auto at = [&](const void* base, long long r, int i) { return E::to_float(static_cast<const T*>(base)[r * p.n + i]); };
@@ -158,11 +148,11 @@ __global__ void __launch_bounds__(kTeamMaxThreads) residual_norm_long_rows_kerne
     mean = 0.f;
     if (kind == kNormLayer) {
       float s = 0.f;
-      for (int i = team.tid; i < p.n; i += team.threads) s += value(i);
+      for (int i = team.tid; i < p.n; i += kTeamMaxThreads) s += value(i);
       mean = team.sum(s, slot) * inv_n;
     }
     float q = 0.f;
-    for (int i = team.tid; i < p.n; i += team.threads) {
+    for (int i = team.tid; i < p.n; i += kTeamMaxThreads) {
       const float d = value(i) - mean;
       q = fmaf(d, d, q);
     }
@@ -190,42 +180,43 @@ __global__ void __launch_bounds__(kTeamMaxThreads) residual_norm_long_rows_kerne
   RowScale s;
   if constexpr (QUANTIZE) {
     uint32_t most = 0;
-    for (int i = team.tid; i < p.n; i += team.threads) most = max(most, magnitude_bits(result(i, total(i))));
+    for (int i = team.tid; i < p.n; i += kTeamMaxThreads) {
+      const float y = result(i, total(i));
+      take_magnitudes<1>(most, &y);
+    }
     s = row_scale_of(team.most(most, 4));
     if (team.tid == 0) p.scale[row] = s.scale;
   }
-  for (int i = team.tid; i < p.n; i += team.threads) {
+  for (int i = team.tid; i < p.n; i += kTeamMaxThreads) {
     const float v = total(i), y = result(i, v);
     if (p.sum) static_cast<T*>(p.sum)[row * p.n + i] = E::from_float(v);
     if constexpr (QUANTIZE) {
-      store_quantized<1>(static_cast<int8_t*>(p.y) + row * p.y_pitch, i, s, &y);
+      (static_cast<int8_t*>(p.y) + row * p.y_pitch)[i] = quantize_value(s, y);
     } else {
       static_cast<T*>(p.y)[row * p.n + i] = E::from_float(y);
     }
   }
 }
 
-template <int VEC, int CNT, int MOST, bool QUANTIZE, bool BF16>
-static void launch_residual_norm(const ResidualNormParams& p, int threads, cudaStream_t stream) {
-  constexpr bool BLOCK = MOST > 32;
-  const long long blocks = BLOCK ? p.rows : (p.rows + kTeamWarpsPerBlock - 1) / kTeamWarpsPerBlock;
-  const int block = BLOCK ? threads : 32 * kTeamWarpsPerBlock;
-  const bool early = blocks_start_early(blocks, block, sm_count(), 2048) || !in_capture(stream);
-  launch_early(&residual_norm_kernel<VEC, CNT, MOST, QUANTIZE, BF16>, dim3(static_cast<unsigned>(blocks)), block, 0, stream, early, 1,
-               p);
+template <int CNT, int THREADS, bool ALIGNED, bool QUANTIZE, bool BF16>
+static void launch_residual_norm(const ResidualNormParams& p, cudaStream_t stream) {
+  constexpr int kBlock = kTeamBlock<THREADS>;
+  const long long blocks = THREADS > 32 ? p.rows : (p.rows + kTeamWarpsPerBlock - 1) / kTeamWarpsPerBlock;
+  const bool early = blocks_start_early(blocks, kBlock, sm_count(), 2048) || !in_capture(stream);
+  launch_early(&residual_norm_kernel<CNT, THREADS, ALIGNED, QUANTIZE, BF16>, dim3(static_cast<unsigned>(blocks)), kBlock, 0, stream, early, 1, p);
 }
 
 template <bool QUANTIZE, bool BF16>
-static void residual_norm_dispatch(const ResidualNormParams& p, bool vector_ok, cudaStream_t stream) {
-  const TeamShape t = team_shape(p.rows, p.n, vector_ok, sm_count());
-  if (t.cnt == 0) {
+static void residual_norm_dispatch(const ResidualNormParams& p, bool lie_well, bool aligned, cudaStream_t stream) {
+  const TeamShape t = team_shape(p.rows, p.n, aligned, sm_count());
+  if (t.cnt == 0 || !lie_well) {
     count_launch();
-    residual_norm_long_rows_kernel<QUANTIZE, BF16><<<static_cast<unsigned>(p.rows), t.threads, 0, stream>>>(p);
+    residual_norm_long_rows_kernel<QUANTIZE, BF16><<<static_cast<unsigned>(p.rows), kTeamMaxThreads, 0, stream>>>(p);
     B200AIT_CUDA_CHECK(cudaGetLastError());
     return;
   }
-  for_team_shape(t, [&](auto vec, auto cnt, auto most) {
-    launch_residual_norm<decltype(vec)::value, decltype(cnt)::value, decltype(most)::value, QUANTIZE, BF16>(p, t.threads, stream);
+  for_team_shape(t, [&](auto cnt, auto threads, auto whole) {
+    launch_residual_norm<decltype(cnt)::value, decltype(threads)::value, decltype(whole)::value, QUANTIZE, BF16>(p, stream);
   });
 }
 
@@ -259,19 +250,20 @@ B200AIT_EXPORT int b200ait_residual_norm(void* sum, void* y, float* y_scale, con
     part(gate, gates, "gate", p.gate_part);
     part(gamma, gammas, "gamma", p.gamma_part);
     part(beta, betas, "beta", p.beta_part);
-    bool vector_ok = n % 8 == 0;
     for (const void* ptr : {x, residual, gate, post_gamma, post_beta, gamma, beta, static_cast<const void*>(sum)})
-      vector_ok = vector_ok && (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0;
-    vector_ok = vector_ok && (quantize ? (reinterpret_cast<uintptr_t>(y) & 7u) == 0 && y_pitch % 8 == 0
-                                       : (reinterpret_cast<uintptr_t>(y) & 15u) == 0);
+      B200AIT_REQUIRE(multiple_of(ptr, 2), "residual_norm: a pointer is not aligned to its type");
+    B200AIT_REQUIRE(multiple_of(y, quantize ? 1 : 2) && multiple_of(y_scale, 4), "residual_norm: a pointer is not aligned to its type");
+    const bool lie_well = quantize ? lie_alike({x, residual, sum}) && multiple_of(y, 8) && y_pitch % 8 == 0 : lie_alike({x, residual, sum, y});
+    bool aligned = n % 8 == 0 && multiple_of(x, 16);
+    for (const void* vector : {gate, post_gamma, post_beta, gamma, beta}) aligned = aligned && multiple_of(vector, 16);
     const bool bf16 = dtype == kDTypeBFloat16;
     if (quantize && bf16)
-      residual_norm_dispatch<true, true>(p, vector_ok, stream);
+      residual_norm_dispatch<true, true>(p, lie_well, aligned, stream);
     else if (quantize)
-      residual_norm_dispatch<true, false>(p, vector_ok, stream);
+      residual_norm_dispatch<true, false>(p, lie_well, aligned, stream);
     else if (bf16)
-      residual_norm_dispatch<false, true>(p, vector_ok, stream);
+      residual_norm_dispatch<false, true>(p, lie_well, aligned, stream);
     else
-      residual_norm_dispatch<false, false>(p, vector_ok, stream);
+      residual_norm_dispatch<false, false>(p, lie_well, aligned, stream);
   });
 }

@@ -1,8 +1,20 @@
-// What the kernels share that hold a row in registers from its one read to its one write: a warp or a block ("team") per row, CNT
-// units of VEC elements a thread, unit i of thread t at t + i * team. Reductions over the row, and the step from fp32 values to
-// signed 8-bit ones with a scale per row.
+// What the kernels share that hold a row in registers from its one read to its one write: a team of THREADS threads (a warp, or
+// a whole block) per row, CNT units of 8 elements a thread, unit i of thread t at t + i * THREADS. Reductions over the row, and the
+// step from fp32 values to signed 8-bit ones with a scale per row.
+//
+// With norms on both sides of a block these kernels are bound by how many instructions a value takes as much as by HBM (8192 x 4096, both
+// norms, to 8 bits: 40 a value and 59 us with THREADS read from the launch and every access checked). So THREADS is known at
+// compile time, which leaves one address per operand and row, only the last unit of a thread can lie past the end of the row, what an
+// operand does to the row is asked once per row, and arithmetic takes two values at a time.
+//
+// ALIGNED: rows start on 16 bytes and hold whole units. Otherwise units are cut where the 16-byte boundaries of the row's memory lie,
+// so that its elements still move 16 bytes at a time (all of the [rows, n] operands of a call lie alike, the host sees to it): the
+// first unit lacks its first `skew` elements, the last one its end, which are read along and left out, and written element by element. Vectors that rows share,
+// and 8-bit results, whose rows start on 16 bytes, then lie off the units: two loads and a shift of the words, or a way through shared
+// memory. Element by element throughout, 8192 x 1001 with both norms took 33 us, 8192 x 5001 to 8 bits 226.
 #pragma once
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.h"
@@ -15,70 +27,168 @@ namespace b200ait {
 constexpr int kTeamMaxThreads = 1024;
 constexpr int kTeamWarpsPerBlock = 8;  // rows of a block where a warp takes a row
 
-// threads of a block whose teams have up to MOST
-template <int MOST>
-constexpr int kTeamBlock = MOST == 32 ? 32 * kTeamWarpsPerBlock : MOST;
+template <int THREADS>
+constexpr int kTeamBlock = THREADS == 32 ? 32 * kTeamWarpsPerBlock : THREADS;
+
+// Eight elements of a piece that reaches over an end of the tensor's memory [lo, hi). Two pieces of a launch do; inlined at every load it
+// filled the instruction cache.
+static __device__ __noinline__ uint4 load_elements(const uint16_t* at, const uint16_t* lo, const uint16_t* hi) {
+  uint32_t e[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = at + j >= lo && at + j < hi ? at[j] : 0u;
+  return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+}
+// The elements from .. to - 1 of a unit, one by one
+static __device__ __noinline__ void store_elements(uint16_t* at, uint4 v, int from, int to) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j >= from && j < to) at[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+}
 
 // A reduction needs one barrier: each has words of its own (`slot`), so no thread can overwrite what another still reads.
-template <bool BLOCK>
+template <int CNT, int THREADS, bool ALIGNED>
 struct RowTeam {
+  static constexpr bool kBlock = THREADS > 32;
   uint32_t (*words)[32];  // [slots][warps], shared
-  int tid, threads;
+  int tid, units, n, skew;
+
+  // `row`: where the row starts in one of the operands that lie alike
+  __device__ __forceinline__ RowTeam(uint32_t (*w)[32], int columns, const void* row)
+      : words(w), tid(kBlock ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x & 31)), n(columns),
+        skew(ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 7) {
+    units = (n + skew + 7) >> 3;
+  }
+  static __device__ __forceinline__ long long row() {
+    return kBlock ? static_cast<long long>(blockIdx.x)
+                  : static_cast<long long>(blockIdx.x) * kTeamWarpsPerBlock + (threadIdx.x >> 5);
+  }
+  __device__ __forceinline__ int unit(int i) const { return tid + i * THREADS; }
+  // (of aligned rows the host takes as few units a thread as the row allows)
+  __device__ __forceinline__ bool has(int i) const { return (ALIGNED && i < CNT - 1) || unit(i) < units; }
+  // element of the row that unit i starts with (negative for the first one of a skewed row), and which of its 8 are the row's
+  __device__ __forceinline__ int first(int i) const { return unit(i) * 8 - skew; }
+  __device__ __forceinline__ int from(int i) const { return max(0, -first(i)); }
+  __device__ __forceinline__ int to(int i) const { return min(8, n - first(i)); }
+  __device__ __forceinline__ bool whole(int i) const { return ALIGNED || (first(i) >= 0 && first(i) + 8 <= n); }
 
   __device__ __forceinline__ float sum(float v, int slot) const {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if constexpr (BLOCK) {
-      const int lane = tid & 31;
-      if (lane == 0) words[slot][tid >> 5] = __float_as_uint(v);
+    if constexpr (kBlock) {
+      if ((tid & 31) == 0) words[slot][tid >> 5] = __float_as_uint(v);
       __syncthreads();
-      v = lane < (threads >> 5) ? __uint_as_float(words[slot][lane]) : 0.f;
+      v = (tid & 31) < THREADS / 32 ? __uint_as_float(words[slot][tid & 31]) : 0.f;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      for (int o = THREADS / 64; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if constexpr (THREADS < 1024) v = __shfl_sync(0xffffffffu, v, 0);
     }
     return v;
   }
   // the largest of unsigned words
   __device__ __forceinline__ uint32_t most(uint32_t v, int slot) const {
     v = __reduce_max_sync(0xffffffffu, v);
-    if constexpr (BLOCK) {
-      const int lane = tid & 31;
-      if (lane == 0) words[slot][tid >> 5] = v;
+    if constexpr (kBlock) {
+      if ((tid & 31) == 0) words[slot][tid >> 5] = v;
       __syncthreads();
-      v = __reduce_max_sync(0xffffffffu, lane < (threads >> 5) ? words[slot][lane] : 0u);
+      v = __reduce_max_sync(0xffffffffu, (tid & 31) < THREADS / 32 ? words[slot][tid & 31] : 0u);
     }
     return v;
   }
+
+  // Eight elements on 16 bytes, in one piece unless they reach over an end of the tensor's memory [lo, hi).
+  template <bool STREAM>
+  static __device__ __forceinline__ uint4 piece(const uint16_t* at, const uint16_t* lo, const uint16_t* hi) {
+    if (ALIGNED || (at >= lo && at + 8 <= hi))
+      return STREAM ? ld_stream(reinterpret_cast<const uint4*>(at)) : *reinterpret_cast<const uint4*>(at);
+    return load_elements(at, lo, hi);
+  }
+  // Unit i of a row of 16-bit elements in a tensor [lo, hi). What is not the row's holds anything (clear_rest).
+  template <bool STREAM>
+  __device__ __forceinline__ uint4 load(const uint16_t* row, const uint16_t* lo, const uint16_t* hi, int i) const {
+    return has(i) ? piece<STREAM>(row - skew + unit(i) * 8, lo, hi) : make_uint4(0, 0, 0, 0);
+  }
+  // The same elements of a row that may lie at another place of 16 bytes than the team's: the two pieces that hold them, shifted by
+  // words and by half a word.
+  __device__ __forceinline__ uint4 load_off(const uint16_t* row, const uint16_t* lo, const uint16_t* hi, int i) const {
+    if (ALIGNED) return load<false>(row, lo, hi, i);
+    if (!has(i)) return make_uint4(0, 0, 0, 0);
+    const uint16_t* at = row + first(i);
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(at) >> 1) & 7;
+    const uint4 a = piece<false>(at - off, lo, hi);
+    if (off == 0) return a;
+    const uint4 b = piece<false>(at - off + 8, lo, hi);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (off & 4) {
+#pragma unroll
+      for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+    }
+    if (off & 2) {
+#pragma unroll
+      for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+    }
+    if (off & 1) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // zeros for what is not the row's
+  __device__ __forceinline__ void clear_rest(float* v, int i) const {
+    if (ALIGNED ? has(i) : has(i) && whole(i)) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (!has(i) || j < from(i) || j >= to(i)) v[j] = 0.f;
+  }
+  template <bool BF16>
+  __device__ __forceinline__ void store(uint16_t* row, int i, const float* v) const {
+    if (!has(i)) return;
+    const uint4 packed = pack8<BF16>(v);
+    if (whole(i)) {
+      reinterpret_cast<uint4*>(row - skew)[unit(i)] = packed;
+      return;
+    }
+    store_elements(row + first(i), packed, from(i), to(i));
+  }
+  // The row as 8-bit values into one that starts on 8 bytes; every thread of the team calls it. The units of a skewed row lie off
+  // those 8 bytes: they go through shared memory (`staged`), where a thread takes its 8 bytes out of the two units that hold them.
+  static constexpr int kStagedBytes = ALIGNED ? 8 : CNT * THREADS * 8 + 8;
+  __device__ __forceinline__ void store_bytes(int8_t* row, const uint2 (&b)[CNT], uint2* staged) const {
+    if constexpr (ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < CNT; ++i)
+        if (has(i)) reinterpret_cast<uint2*>(row)[unit(i)] = b[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < CNT; ++i) staged[unit(i)] = b[i];
+      if constexpr (kBlock) {
+        __syncthreads();
+      } else {
+        __syncwarp();
+      }
+      const int shift = 8 * skew;
+#pragma unroll
+      for (int i = 0; i < CNT; ++i) {
+        const int g = unit(i), left = n - 8 * g;
+        if (left <= 0) continue;
+        const uint2 lo = staged[g], hi = staged[g + 1];  // (what is behind the last unit is not used)
+        uint64_t v = (static_cast<uint64_t>(lo.y) << 32 | lo.x) >> shift;
+        if (skew != 0) v |= (static_cast<uint64_t>(hi.y) << 32 | hi.x) << (64 - shift);
+        if (left >= 8) {
+          reinterpret_cast<uint64_t*>(row)[g] = v;
+        } else {
+          for (int j = 0; j < left; ++j) row[8 * g + j] = static_cast<int8_t>(v >> (8 * j));
+        }
+      }
+    }
+  }
 };
 
-// VEC elements as they lie in memory
-template <int VEC>
-struct RawUnit;
-template <>
-struct RawUnit<8> {
-  using Type = uint4;
-  static __device__ __forceinline__ uint4 zero() { return make_uint4(0, 0, 0, 0); }
-};
-template <>
-struct RawUnit<1> {
-  using Type = uint16_t;
-  static __device__ __forceinline__ uint16_t zero() { return 0; }
-};
-template <int VEC, bool BF16>
-__device__ __forceinline__ void unpack_unit(const typename RawUnit<VEC>::Type& raw, float* f) {
-  if constexpr (VEC == 8) {
-    unpack8<BF16>(raw, f);
-  } else {
-    f[0] = Elem16<BF16>::to_float(*reinterpret_cast<const typename Elem16<BF16>::T*>(&raw));
-  }
-}
-template <int VEC, bool BF16>
-__device__ __forceinline__ void store_unit(void* base, long long unit, const float* f) {
-  if constexpr (VEC == 8) {
-    static_cast<uint4*>(base)[unit] = pack8<BF16>(f);
-  } else {
-    static_cast<typename Elem16<BF16>::T*>(base)[unit] = Elem16<BF16>::from_float(f[0]);
-  }
+// Arithmetic two values at a time
+template <int N, class F>
+__device__ __forceinline__ void by_pairs(float* v, F&& f) {  // v[j], v[j + 1] = f(pair, j)
+#pragma unroll
+  for (int j = 0; j < N; j += 2) unpack2(f(pack2(v[j], v[j + 1]), j), v[j], v[j + 1]);
 }
 
 // ------------------------------------------------------------------------------------------------ 8-bit values
@@ -90,8 +200,8 @@ __device__ __forceinline__ void store_unit(void* base, long long unit, const flo
 // own size from them (both mantissas have at most 11 bits), sixteen steps of fp32. Adding 1.5 * 2^23 rounds to a whole number, ties to
 // even, and leaves it in the low bits. Five packed instructions for two values; a division would take eight for each.
 //
-// The largest |v| is found among the bit patterns without their sign, as integers: it has no trouble with values under 2^-126,
-// which the compiler's arithmetic here takes for zero, and infinities and NaN come out on top.
+// The largest |v| is looked for without flushing values under 2^-126 to zero, as the compiler's arithmetic here would, and in such a way
+// that NaN comes out on top; across threads it is compared as an integer (the bits of a magnitude are ordered as it is).
 struct RowScale {
   float scale;                // what one step of q is worth
   float prescale, amax, inv, back;  // amax after prescaling, 127 / amax, 1 / amax
@@ -116,83 +226,79 @@ __device__ __forceinline__ RowScale row_scale_of(uint32_t amax_bits) {
   s.back = __fdiv_rn(1.f, s.amax);
   return s;
 }
-__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-// N values (N even) -> N bytes in N / 4 words (one value: N = 1)
+// the bits of the larger of `most` and every |v|
 template <int N>
-__device__ __forceinline__ void quantize_values(const RowScale& s, const float* v, uint32_t* words) {
-  static_assert(N == 1 || N % 4 == 0, "whole words");
-  uint32_t b[N == 1 ? 2 : N];
-  const uint64_t inv = pack2(s.inv, s.inv), back = pack2(s.back, s.back), less = pack2(-s.amax, -s.amax);
-  const uint64_t steps = pack2(127.f, 127.f), whole = pack2(12582912.f, 12582912.f);
+__device__ __forceinline__ void take_magnitudes(uint32_t& most, const float* v) {
+  float m = __uint_as_float(most);
 #pragma unroll
-  for (int j = 0; j < N; j += 2) {
-    float v0 = v[j], v1 = N == 1 ? 0.f : v[j + 1];
-    if (s.prescale != 1.f) v0 = mul_exact(v0, s.prescale), v1 = mul_exact(v1, s.prescale);
-    const uint64_t x = pack2(v0, v1);
-    const uint64_t r0 = mul2(x, inv), r = fma2(fma2(r0, less, mul2(x, steps)), back, r0);
-    float m0, m1;
-    unpack2(add2(r, whole), m0, m1);
-    b[j] = __float_as_uint(m0), b[j + 1] = __float_as_uint(m1);
-  }
-  if constexpr (N == 1) {
-    words[0] = s.flat ? 0u : b[0] & 0xffu;
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; j += 4) {
-      const uint32_t lo = __byte_perm(b[j], b[j + 1], 0x0040), hi = __byte_perm(b[j + 2], b[j + 3], 0x0040);
-      words[j / 4] = s.flat ? 0u : __byte_perm(lo, hi, 0x5410);
-    }
-  }
+  for (int j = 0; j < N; j += 2)
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(v[j]), "f"(v[N == 1 ? j : j + 1]));
+  most = __float_as_uint(m);
 }
-template <int VEC>
-__device__ __forceinline__ void store_quantized(int8_t* row, long long unit, const RowScale& s, const float* v) {
-  uint32_t w[VEC == 8 ? 2 : 1];
-  quantize_values<VEC>(s, v, w);
-  if constexpr (VEC == 8) {
-    reinterpret_cast<uint2*>(row)[unit] = make_uint2(w[0], w[1]);
-  } else {
-    row[unit] = static_cast<int8_t>(w[0]);
-  }
+
+// two values as whole numbers, in the low bytes of the words
+__device__ __forceinline__ void quantize_pair(const RowScale& s, float v0, float v1, uint32_t& b0, uint32_t& b1) {
+  if (s.prescale != 1.f) v0 = mul_exact(v0, s.prescale), v1 = mul_exact(v1, s.prescale);
+  const uint64_t x = pack2(v0, v1), r0 = mul2(x, pack2(s.inv, s.inv));
+  const uint64_t rest = fma2(r0, pack2(-s.amax, -s.amax), mul2(x, pack2(127.f, 127.f)));
+  float m0, m1;
+  unpack2(add2(fma2(rest, pack2(s.back, s.back), r0), pack2(12582912.f, 12582912.f)), m0, m1);
+  b0 = s.flat ? 0u : __float_as_uint(m0), b1 = s.flat ? 0u : __float_as_uint(m1);
+}
+__device__ __forceinline__ uint2 quantize_unit(const RowScale& s, const float* v) {
+  uint32_t b[8];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) quantize_pair(s, v[j], v[j + 1], b[j], b[j + 1]);
+  auto word = [&](int j) { return __byte_perm(__byte_perm(b[j], b[j + 1], 0x0040), __byte_perm(b[j + 2], b[j + 3], 0x0040), 0x5410); };
+  return make_uint2(word(0), word(4));
+}
+__device__ __forceinline__ int8_t quantize_value(const RowScale& s, float v) {
+  uint32_t b, unused;
+  quantize_pair(s, v, 0.f, b, unused);
+  return static_cast<int8_t>(b);
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// How a row of n elements is laid over threads: `cnt` units of `vec` elements each (0: the row is too long and is walked), by a warp
-// (most = 32) or by a block of `threads` whose kernel is built for up to `most`.
+// How a row of n elements is laid over threads: `cnt` units each; 0: the row is too long and is walked.
 struct TeamShape {
-  int vec, cnt, threads, most;
+  int cnt, threads;
+  bool aligned;
 };
-inline TeamShape team_shape(long long rows, long long n, bool vector_ok, int sms) {
-  auto shape = [](int vec, long long units, long long per) {
-    const int t = static_cast<int>(std::max<long long>(32, ((units + per - 1) / per + 31) / 32 * 32));
-    const int cnt = static_cast<int>(std::max<long long>(1, (units + t - 1) / t));
-    return TeamShape{vec, cnt, t, t == 32 && vec == 8 ? 32 : t <= 256 ? 256 : t <= 512 ? 512 : 1024};
-  };
-  if (!vector_ok) {
-    if (n > 32ll * kTeamMaxThreads) return TeamShape{1, 0, kTeamMaxThreads, kTeamMaxThreads};
-    TeamShape t = shape(1, n, n <= 8ll * kTeamMaxThreads ? 8 : 32);
-    t.cnt = n <= 8ll * kTeamMaxThreads ? 8 : 32, t.most = kTeamMaxThreads;
-    return t;
-  }
-  const long long units = n / 8;
-  if (units > 4ll * kTeamMaxThreads) return TeamShape{8, 0, kTeamMaxThreads, kTeamMaxThreads};
+inline TeamShape team_shape(long long rows, long long n, bool aligned, int sms) {
+  const long long units = aligned ? n / 8 : (n + 14) / 8;
+  if (units > (aligned ? 4 : 2) * kTeamMaxThreads) return TeamShape{0, kTeamMaxThreads, aligned};
   // A few rows are a matter of latency: a unit a thread. Many are one of bytes in flight: up to four.
-  return shape(8, units, rows <= 2ll * sms && units <= kTeamMaxThreads ? 1 : 4);
+  // (Skewed rows take registers: two.)
+  const long long per = rows <= 2ll * sms && units <= kTeamMaxThreads ? 1 : aligned ? 4 : 2;
+  int threads = 32;
+  while (threads * per < units) threads *= 2;
+  const int cnt = static_cast<int>((units + threads - 1) / threads);
+  return TeamShape{cnt, threads, aligned};
 }
+// Do these operands of rows at a pitch of whole elements lie alike: at the same place of 16 bytes in every row?
+inline bool lie_alike(std::initializer_list<const void*> operands) {
+  const void* one = nullptr;
+  for (const void* p : operands) {
+    if (p == nullptr) continue;
+    if (one != nullptr && ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(one)) & 15u) != 0) return false;
+    one = p;
+  }
+  return true;
+}
+inline bool multiple_of(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// Calls `launch` with (VEC, CNT, MOST) as compile-time numbers. Of block-wide shapes with 16-byte units only these come about: one unit
-// a thread, or four, and three where a block has 64 or 96 threads.
-template <int N>
-using TeamInt = std::integral_constant<int, N>;
+// Calls `launch` with (CNT, THREADS, ALIGNED) as compile-time numbers.
 template <class F>
 inline void for_team_shape(const TeamShape& t, F&& launch) {
-  switch (t.vec * 100000 + t.most * 10 + (t.vec == 8 ? t.cnt : t.cnt == 32 ? 1 : 0)) {
-#define B200AIT_TEAM(VEC, CNT, MOST) \
-  case (VEC) * 100000 + (MOST) * 10 + ((VEC) == 8 ? (CNT) : (CNT) == 32 ? 1 : 0): return launch(TeamInt<VEC>{}, TeamInt<CNT>{}, TeamInt<MOST>{});
-    B200AIT_TEAM(8, 1, 32) B200AIT_TEAM(8, 2, 32) B200AIT_TEAM(8, 3, 32) B200AIT_TEAM(8, 4, 32)
-    B200AIT_TEAM(8, 1, 256) B200AIT_TEAM(8, 3, 256) B200AIT_TEAM(8, 4, 256)
-    B200AIT_TEAM(8, 1, 512) B200AIT_TEAM(8, 4, 512) B200AIT_TEAM(8, 1, 1024) B200AIT_TEAM(8, 4, 1024)
-    B200AIT_TEAM(1, 8, 1024) B200AIT_TEAM(1, 32, 1024)
+  switch (t.cnt * 10000 + t.threads + (t.aligned ? 0 : 1)) {
+#define B200AIT_TEAM(CNT, THREADS, ALIGNED)            \
+  case (CNT) * 10000 + (THREADS) + ((ALIGNED) ? 0 : 1): \
+    return launch(std::integral_constant<int, CNT>{}, std::integral_constant<int, THREADS>{}, std::integral_constant<bool, ALIGNED>{});
+#define B200AIT_TEAMS(THREADS)                                                                                   \
+  B200AIT_TEAM(1, THREADS, true) B200AIT_TEAM(2, THREADS, true) B200AIT_TEAM(3, THREADS, true) B200AIT_TEAM(4, THREADS, true) \
+  B200AIT_TEAM(1, THREADS, false) B200AIT_TEAM(2, THREADS, false)
+    B200AIT_TEAMS(32) B200AIT_TEAMS(64) B200AIT_TEAMS(128) B200AIT_TEAMS(256) B200AIT_TEAMS(512) B200AIT_TEAMS(1024)
+#undef B200AIT_TEAMS
 #undef B200AIT_TEAM
   }
   throw Error("no kernel for rows of this length");

@@ -3,14 +3,17 @@
 // and took the host 12, of which the launch itself is 3 (here 6; a softmax 7 -> 4.3, seven row-wise calls 70 -> 28; run_with_tensors of an
 // encoder layer at batch 1 70 -> 55 with the GPU's 45).
 //
-// Every function takes plain calls only (exact torch.Tensor or Parameter objects on the GPU, contiguous, shapes that fit) and
+// Every function takes plain calls only (exact torch.Tensor or Parameter objects on the GPU, contiguous or, of those read as rows, rows at one
+// distance, shapes that fit) and
 // returns None for anything else; the Python code behind it then runs as if this module were not there, and is the one
 // place that refuses calls and says why. Nothing is kept from one call for the next.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -39,11 +42,14 @@ struct Library {
   decltype(&b200ait_permute) permute;
   decltype(&b200ait_last_error) last_error;
   decltype(&AITemplateModelContainerRun) run;
+  decltype(&b200ait_gemm_rcr_i8) gemm_rcr_i8;
+  decltype(&b200ait_quantize_rows) quantize_rows;
+  decltype(&b200ait_residual_norm) residual_norm;
 } lib;
 PyTypeObject* parameter_type = nullptr;  // torch.nn.Parameter
 
-// A tensor argument: null if the object is no plain tensor on the GPU, contiguous.
-const at::Tensor* plain(PyObject* o) {
+// A tensor argument: null if the object is no plain tensor on the GPU.
+const at::Tensor* strided(PyObject* o) {
   if (Py_TYPE(o) != reinterpret_cast<PyTypeObject*>(THPVariableClass) && Py_TYPE(o) != parameter_type) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   // (a conjugated or negated view, a functorch wrapper or a fake tensor has no memory of its own to hand over)
@@ -52,7 +58,12 @@ const at::Tensor* plain(PyObject* o) {
                                                                      c10::DispatchKey::FuncTorchGradWrapper,
                                                                      c10::DispatchKey::Functionalize, c10::DispatchKey::Python})))
     return nullptr;
-  return t.is_contiguous() ? &t : nullptr;
+  return &t;
+}
+// ... and contiguous
+const at::Tensor* plain(PyObject* o) {
+  const at::Tensor* t = strided(o);
+  return t != nullptr && t->is_contiguous() ? t : nullptr;
 }
 // an optional one: false if it is neither None nor plain
 bool optional_plain(PyObject* o, const at::Tensor** t) {
@@ -370,6 +381,170 @@ PyObject* permute(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   });
 }
 
+// Elements from row to row of a tensor read as rows of its last dim (a single row: its length); -1 where they are at no one distance.
+int64_t row_pitch(const at::Tensor& t) {
+  const int64_t n = t.size(-1);
+  if (n > 1 && t.stride(-1) != 1) return -1;
+  int64_t pitch = -1, step = 0;
+  for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (pitch < 0)
+      pitch = t.stride(d);
+    else if (t.stride(d) != step)
+      return -1;
+    step = t.stride(d) * t.size(d);
+  }
+  return pitch < 0 ? n : pitch < n ? -1 : pitch;
+}
+bool on_current_device(std::initializer_list<const at::Tensor*> tensors) {
+  const auto here = c10::cuda::current_device();
+  for (const at::Tensor* t : tensors)
+    if (t != nullptr && t->get_device() != here) return false;
+  return true;
+}
+int64_t padded(int64_t n) { return (n + 15) / 16 * 16; }
+// int8 of like's shape but rows of n, which start on 16 bytes
+at::Tensor int8_rows(const at::Tensor& like, int64_t n) {
+  std::vector<int64_t> shape(like.sizes().begin(), like.sizes().end());
+  shape.back() = padded(n);
+  at::Tensor q = at::empty(shape, like.options().dtype(at::kChar));
+  return n == shape.back() ? q : q.narrow(-1, 0, n);
+}
+at::Tensor row_scales(const at::Tensor& like) {
+  return at::empty(like.sizes().slice(0, static_cast<size_t>(like.dim() - 1)), like.options().dtype(at::kFloat));
+}
+PyObject* tuple_of(std::initializer_list<at::Tensor> tensors) {
+  PyObject* result = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : tensors)
+    if (result) PyTuple_SET_ITEM(result, i++, THPVariable_Wrap(t));
+  return result;
+}
+
+// quantize_rows(x, activation code, gated)
+PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    int64_t activation;
+    const at::Tensor* x = n_args == 3 ? strided(args[0]) : nullptr;
+    if (!x || x->dim() < 1 || x->numel() == 0 || dtype_code(*x) == 0 || !as_int(args[1], &activation) || !PyBool_Check(args[2]) ||
+        !on_current_device({x}))
+      return unhandled();
+    const bool gated = args[2] == Py_True;
+    const int64_t columns = x->size(-1), n = gated ? columns / 2 : columns, pitch = row_pitch(*x);
+    if (pitch < 0 || (gated && columns % 2 != 0)) return unhandled();
+    at::Tensor q = int8_rows(*x, n), scale = row_scales(*x);
+    const b200ait_stream_t stream = current_stream();
+    if (unlocked([&] {
+          return lib.quantize_rows(q.data_ptr(), static_cast<float*>(scale.data_ptr()), pointer(x), x->numel() / columns, n, pitch,
+                                   padded(n), static_cast<int>(activation), gated, dtype_code(*x), stream);
+        }))
+      return failed("b200ait_quantize_rows");
+    return tuple_of({q, scale});
+  });
+}
+
+// gemm_rcr_i8(x, w, w_scale, x_scale, bias, d0, d1, epilogue code, dtype code or 0, tile_n)
+PyObject* gemm_rcr_i8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 10) return unhandled();
+    const at::Tensor *x = strided(args[0]), *w = strided(args[1]), *w_scale = plain(args[2]), *x_scale, *bias, *d0, *d1;
+    int64_t epilogue, dtype, tile_n;
+    if (!x || !w || !w_scale || !optional_plain(args[3], &x_scale) || !optional_plain(args[4], &bias) || !optional_plain(args[5], &d0) ||
+        !optional_plain(args[6], &d1) || !as_int(args[7], &epilogue) || !as_int(args[8], &dtype) || !as_int(args[9], &tile_n))
+      return unhandled();
+    if (x->dim() < 1 || w->dim() != 2 || x->numel() == 0 || w->numel() == 0 || w->size(1) != x->size(-1) ||
+        w->scalar_type() != at::kChar || !on_current_device({x, w, w_scale, x_scale, bias, d0, d1}))
+      return unhandled();
+    const int64_t n = w->size(0), k = w->size(1), m = x->numel() / k, ldb = row_pitch(*w);
+    int64_t lda = row_pitch(*x);
+    if (lda < 0 || ldb < 0) return unhandled();
+    const bool has_d0 = ((epilogue >> 4) & 3) != 0, has_d1 = ((epilogue >> 6) & 3) != 0;
+    if (has_d0 != (d0 != nullptr) || has_d1 != (d1 != nullptr)) return unhandled();
+    const at::ScalarType given = x->scalar_type() != at::kChar ? x->scalar_type()
+                                 : d0 != nullptr               ? d0->scalar_type()
+                                 : bias != nullptr             ? bias->scalar_type()
+                                                               : at::kHalf;
+    const at::ScalarType type = dtype == 0 ? given : dtype == dtype_code(*x) ? x->scalar_type()
+                                : dtype == static_cast<int>(AITemplateDtype::kHalf) ? at::kHalf : at::kBFloat16;
+    if (type != at::kHalf && type != at::kBFloat16) return unhandled();
+    // the operands in `type`, of the result's shape
+    std::vector<int64_t> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = n;
+    for (const at::Tensor* d : {d0, d1})
+      if (d != nullptr && (d->scalar_type() != type || d->sizes() != c10::IntArrayRef(shape))) return unhandled();
+    if (bias != nullptr && (bias->scalar_type() != type || bias->dim() != 1 || bias->size(0) != n)) return unhandled();
+    if (w_scale->scalar_type() != at::kFloat || w_scale->dim() != 1 || w_scale->size(0) != n) return unhandled();
+    const b200ait_stream_t stream = current_stream();
+    at::Tensor q, scale;
+    if (x->scalar_type() == at::kChar) {
+      if (!x_scale || x_scale->scalar_type() != at::kFloat ||
+          x_scale->sizes() != x->sizes().slice(0, static_cast<size_t>(x->dim() - 1)))
+        return unhandled();
+    } else {
+      if (x_scale || dtype_code(*x) == 0) return unhandled();
+      q = at::empty({m, padded(k)}, x->options().dtype(at::kChar)), scale = row_scales(*x);
+      if (unlocked([&] {
+            return lib.quantize_rows(q.data_ptr(), static_cast<float*>(scale.data_ptr()), pointer(x), m, k, lda, padded(k), 0, 0,
+                                     dtype_code(*x), stream);
+          }))
+        return failed("b200ait_quantize_rows");
+      lda = padded(k);
+    }
+    at::Tensor y = at::empty(shape, x->options().dtype(type));
+    const void* a = q.defined() ? q.data_ptr() : pointer(x);
+    const float* a_scale = static_cast<const float*>(scale.defined() ? scale.data_ptr() : pointer(x_scale));
+    if (unlocked([&] {
+          return lib.gemm_rcr_i8(a, a_scale, pointer(w), static_cast<const float*>(pointer(w_scale)), pointer(bias), pointer(d0),
+                                 pointer(d1), y.data_ptr(), m, n, k, m == 1 ? padded(k) : lda, n == 1 ? padded(k) : ldb, n, n,
+                                 static_cast<int>(epilogue), dtype_code(y), static_cast<int>(tile_n), stream);
+        }))
+      return failed("b200ait_gemm_rcr_i8");
+    return THPVariable_Wrap(std::move(y));
+  });
+}
+
+// residual_norm(x, residual, gate, post_gamma, post_beta, gamma, beta, post norm code, norm code, residual_scale, eps, quantize)
+PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 12) return unhandled();
+    const at::Tensor *x = plain(args[0]), *t[6];  // residual, gate, post_gamma, post_beta, gamma, beta
+    int64_t post, norm;
+    double residual_scale, eps;
+    if (!x || x->dim() < 1 || x->numel() == 0 || dtype_code(*x) == 0) return unhandled();
+    for (int i = 0; i < 6; ++i)
+      if (!optional_plain(args[1 + i], &t[i]) || (t[i] != nullptr && t[i]->scalar_type() != x->scalar_type())) return unhandled();
+    if (!as_int(args[7], &post) || !as_int(args[8], &norm) || !as_double(args[9], &residual_scale) || !as_double(args[10], &eps) ||
+        !PyBool_Check(args[11]) || !on_current_device({x, t[0], t[1], t[2], t[3], t[4], t[5]}))
+      return unhandled();
+    const int64_t n = x->size(-1), rows = x->numel() / n;
+    int64_t parts[6] = {1, 1, 1, 1, 1, 1};
+    if (t[0] != nullptr && t[0]->sizes() != x->sizes()) return unhandled();
+    for (int i = 1; i < 6; ++i) {
+      if (t[i] == nullptr) continue;
+      const bool shared = i == 2 || i == 3;  // post_gamma, post_beta
+      if (t[i]->dim() < 1 || t[i]->dim() > (shared ? 1 : 2) || t[i]->size(-1) != n) return unhandled();
+      parts[i] = t[i]->dim() == 2 ? t[i]->size(0) : 1;
+      if (parts[i] == 0 || rows % parts[i] != 0) return unhandled();
+    }
+    if (post == 0 && (t[2] != nullptr || t[3] != nullptr)) return unhandled();
+    const bool quantize = args[11] == Py_True;
+    at::Tensor total = at::empty_like(*x), y, scale;
+    if (quantize)
+      y = int8_rows(*x, n), scale = row_scales(*x);
+    else
+      y = at::empty_like(*x);
+    const b200ait_stream_t stream = current_stream();
+    if (unlocked([&] {
+          return lib.residual_norm(total.data_ptr(), y.data_ptr(), quantize ? static_cast<float*>(scale.data_ptr()) : nullptr, pointer(x),
+                                   pointer(t[0]), pointer(t[1]), pointer(t[2]), pointer(t[3]), pointer(t[4]), pointer(t[5]), rows, n,
+                                   parts[1], parts[4], parts[5], padded(n), static_cast<int>(post), static_cast<int>(norm),
+                                   static_cast<float>(residual_scale), static_cast<float>(eps), dtype_code(*x), stream);
+        }))
+      return failed("b200ait_residual_norm");
+    return quantize ? tuple_of({total, y, scale}) : tuple_of({total, y});
+  });
+}
+
 // One side (inputs or outputs) of a run, in the order of the model's indexes.
 struct Side {
   std::vector<AITData> data;
@@ -492,6 +667,9 @@ PyMethodDef methods[] = {B200AIT_METHOD(bind),
                          B200AIT_METHOD(split),
                          B200AIT_METHOD(permute),
                          B200AIT_METHOD(run_model),
+                         B200AIT_METHOD(quantize_rows),
+                         B200AIT_METHOD(gemm_rcr_i8),
+                         B200AIT_METHOD(residual_norm),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "torch_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -434,6 +434,9 @@ def quantize_rows(x: torch.Tensor, activation: str = "identity", gated: bool = F
     feed-forward's first product, and v = act(x[..., :n]) * x[..., n:]. A row of zeros gets scale 0; a row with an infinity or
     a NaN in it gets scale NaN and zeros. Rows of x may lie apart. Where n is not a multiple of 16, q is a view of rows padded
     to 16 bytes, so that the product can read them with the tensor cores."""
+    y = (_calls or _native()).quantize_rows(x, UNARY.get(activation), gated)
+    if y is not None:
+        return y
     _check_here("quantize_rows", x=x)
     if activation not in UNARY:
         raise ValueError(f"quantize_rows: unknown activation {activation}")
@@ -463,6 +466,10 @@ def gemm_rcr_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale
     x_scale: its rows are then quantised on the way. Sums are exact (K up to 131071). The epilogues are gemm_rcr's. `dtype`: of
     y, bias, d0 and d1 (default: x's if that has 16 bits, else d0's or the bias's, else float16). Rows of x and w may lie apart;
     the tensor cores want them to start on 16 bytes (a pitch that is a multiple of 16), other rows take a slower kernel."""
+    y = (_calls or _native()).gemm_rcr_i8(x, w, w_scale, x_scale, bias, d0, d1, _EPILOGUE_CODES.get(epilogue),
+                                          0 if dtype is None else _DTYPE_CODE.get(dtype), tile_n)
+    if y is not None:
+        return y
     what = "gemm_rcr_i8"
     _check_here(what, x=x, w=w, w_scale=w_scale, x_scale=x_scale, bias=bias, d0=d0, d1=d1)
     if w.dim() != 2 or x.dim() < 1 or w.shape[1] != x.shape[-1]:
@@ -526,6 +533,10 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, gate
     norm and post_norm: "layer" or "rms", post_norm None for no norm after the block. residual, gate, the gammas and the betas may be
     left out. post_gamma and post_beta are [N]; gate, gamma and beta [N] or [G, N], a vector for each of G equal parts of the rows
     (a gate per sample). y comes of the unrounded total."""
+    y = (_calls or _native()).residual_norm(x, residual, gate, post_gamma, post_beta, gamma, beta, NORMS.get(post_norm),
+                                            NORMS.get(norm) or None, residual_scale, eps, quantize)
+    if y is not None:
+        return y
     what = "residual_norm"
     operands = dict(x=x, residual=residual, gate=gate, post_gamma=post_gamma, post_beta=post_beta, gamma=gamma, beta=beta)
     _check_here(what, **operands)

@@ -415,6 +415,83 @@ def test_residual_norm_rows_stand_alone():
         assert bool(torch.isnan(kernels.residual_norm(x, **o)[1][3]).all())
 
 
+def _at(t, elements):
+    """a contiguous copy of t that starts `elements` elements after a 16-byte boundary"""
+    store = torch.full((t.numel() + elements + 8,), 7.0, dtype=t.dtype, device=t.device)
+    store[elements:elements + t.numel()] = t.reshape(-1)
+    return store[elements:elements + t.numel()].view(t.shape)
+
+
+@pytest.mark.parametrize("n", [8, 9, 31, 264, 1001, 1280, 4100])
+@pytest.mark.parametrize("place", [0, 1, 4, 7])
+def test_rows_anywhere_in_memory(n, place):
+    """The result does not depend on where the operands lie, alike or each at a place of its own."""
+    rows = 21
+    x, o = _norm_operands(rows, n, torch.bfloat16, n, 3, "layer", "rms")
+    want = kernels.residual_norm(x, quantize=True, **o), kernels.residual_norm(x, **o)
+    for moved in (("residual",), ("gamma",), ("gate", "post_beta"), ("residual", "gate", "gamma", "beta", "post_gamma", "post_beta")):
+        p = {k: _at(v, (place + i) % 8) if k in moved else v for i, (k, v) in enumerate(o.items())}
+        got = kernels.residual_norm(_at(x, place), quantize=True, **p), kernels.residual_norm(_at(x, place), **p)
+        for a, b in zip(want, got):
+            for c, d in zip(a, b):
+                if c.dtype == torch.int8:
+                    assert float((c != d).double().mean()) < 0.01 and int((c.int() - d.int()).abs().max()) <= 1
+                else:  # (sums in another order)
+                    assert torch.allclose(c.float(), d.float(), rtol=2.0 ** -7, atol=1e-5)
+    v = x[:, :n // 2 * 2]
+    for gated in (False, True):
+        if gated and n < 16:
+            continue
+        a = kernels.quantize_rows(v.contiguous(), "relu", gated=gated)
+        b = kernels.quantize_rows(_at(v.contiguous(), place), "relu", gated=gated)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_results_stay_in_their_rows():
+    """What lies between and around the rows of q, total and y stays as it was, wherever the rows end."""
+    from aitemplate_b200 import _lib
+
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    for n in (1, 7, 8, 9, 15, 100, 257, 1003, 2049, 4104):
+        pitch = (n + 15) // 16 * 16 + 16
+        x = torch.randn(5, n, generator=_gen(n), device="cuda").to(torch.float16)
+        q = torch.full((7, pitch), 99, dtype=torch.int8, device="cuda")
+        scale = torch.full((7,), 5.0, device="cuda")
+        _lib.check(lib.b200ait_quantize_rows(q[1:].data_ptr(), scale[1:].data_ptr(), x.data_ptr(), 5, n, n, pitch, 0, 0, 1, stream), "")
+        want, ws = kernels.quantize_rows(x)
+        assert torch.equal(q[1:6, :n], want) and torch.equal(scale[1:6], ws)
+        assert bool((q[1:6, n:] == 99).all()) and bool((q[[0, 6]] == 99).all()) and scale[0] == 5 and scale[6] == 5
+        total, y = (torch.full((5 * n + 32,), 99.0, dtype=torch.float16, device="cuda") for _ in range(2))
+        for lead in (8, 3):
+            total.fill_(99), y.fill_(99), q.fill_(99), scale.fill_(5)
+            a, b = _at(x, lead), _at(x, lead)
+            _lib.check(lib.b200ait_residual_norm(total[lead:].data_ptr(), y[lead:].data_ptr(), None, a.data_ptr(), b.data_ptr(), None, None,
+                                                 None, None, None, 5, n, 1, 1, 1, 0, 0, 2, 1.0, 1e-5, 1, stream), "")
+            for t in (total, y):
+                assert bool((t[:lead] == 99).all()) and bool((t[lead + 5 * n:] == 99).all())
+            assert torch.equal(total[lead:lead + 5 * n].view(5, n), x + x)
+            _lib.check(lib.b200ait_residual_norm(None, q[1:].data_ptr(), scale[1:].data_ptr(), a.data_ptr(), b.data_ptr(), None, None,
+                                                 None, None, None, 5, n, 1, 1, 1, pitch, 0, 2, 1.0, 1e-5, 1, stream), "")
+            assert bool((q[1:6, n:] == 99).all()) and bool((q[[0, 6]] == 99).all()) and scale[0] == 5 and scale[6] == 5
+            assert bool((q[1:6, :n].abs().amax(1) == 127).all())
+
+
+def test_residual_norm_in_place():
+    """total may be written over the residual, or over x."""
+    from aitemplate_b200 import _lib
+
+    for n in (1000, 1001, 40000):
+        x, o = _norm_operands(9, n, torch.float16, n, 1, None, "layer")
+        want = kernels.residual_norm(x, **o)
+        for over in ("residual", "x"):
+            a, r = x.clone(), o["residual"].clone()
+            y = torch.empty_like(x)
+            _lib.check(_lib.load().b200ait_residual_norm(
+                (r if over == "residual" else a).data_ptr(), y.data_ptr(), None, a.data_ptr(), r.data_ptr(), o["gate"].data_ptr(), None, None,
+                o["gamma"].data_ptr(), o["beta"].data_ptr(), 9, n, 1, 1, 1, 0, 0, 1, 0.75, 1e-5, 1, torch.cuda.current_stream().cuda_stream), "")
+            assert torch.equal(r if over == "residual" else a, want[0]) and torch.equal(y, want[1])
+
+
 def test_residual_norm_leading_dims_and_empty():
     x, o = _norm_operands(24, 256, torch.float16, 2, 2, None, "rms")
     s, y = kernels.residual_norm(x, **o)
