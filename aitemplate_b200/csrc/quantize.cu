@@ -29,12 +29,13 @@ __global__ void __launch_bounds__(kTeamBlock<THREADS>) quantize_rows_kernel(cons
   const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.x_pitch;
   const uint16_t* lo = static_cast<const uint16_t*>(p.x);
   const uint16_t* hi = lo + (p.rows - 1) * p.x_pitch + (GATED ? 2 * p.n : p.n);
+  const bool inner = row > 0 && row < p.rows - 1;
   const Team team(words, p.n, x);
   uint4 raw[CNT], up[GATED ? CNT : 1];
 #pragma unroll
   for (int i = 0; i < CNT; ++i) {
-    raw[i] = team.template load<true>(x, lo, hi, i);
-    if (GATED) up[i] = ALIGNED ? team.template load<true>(x + p.n, lo, hi, i) : team.load_off(x + p.n, lo, hi, i);
+    raw[i] = team.load(x, inner, lo, hi, i);
+    if (GATED) up[i] = team.template load_off<true>(x + p.n, i);
   }
   float v[CNT * 8];
 #pragma unroll

@@ -64,11 +64,12 @@ __global__ void __launch_bounds__(kTeamBlock<THREADS>) residual_norm_kernel(cons
   const long long at = row * p.n, all = p.rows * p.n;
   const Team team(words, p.n, static_cast<const uint16_t*>(p.x) + at);
   const float inv_n = 1.f / static_cast<float>(p.n);
+  const bool inner = row > 0 && row < p.rows - 1;
   uint4 xr[CNT], rr[CNT];
   auto fetch = [&](const void* tensor, uint4 (&raw)[CNT]) {
     const uint16_t* t = static_cast<const uint16_t*>(tensor);
 #pragma unroll
-    for (int i = 0; i < CNT; ++i) raw[i] = team.template load<true>(t + at, t, t + all, i);
+    for (int i = 0; i < CNT; ++i) raw[i] = team.load(t + at, inner, t, t + all, i);
   };
   fetch(p.x, xr);
   if (p.residual != nullptr) fetch(p.residual, rr);
@@ -79,15 +80,13 @@ __global__ void __launch_bounds__(kTeamBlock<THREADS>) residual_norm_kernel(cons
   };
 #pragma unroll
   for (int i = 0; i < CNT; ++i) unpack8<BF16>(xr[i], &v[i * 8]);
-  // every pair of values with the same two of vector r of those that `part` rows share each
-  auto with = [&](const void* vectors, long long r, long long part, auto&& f) {
-    const uint16_t* t = static_cast<const uint16_t*>(vectors);
-    const uint16_t* vector = t + r * p.n;
-    const uint16_t* end = t + (p.rows / part) * p.n;
+  // every pair of values with the same two of vector r of those that rows share
+  auto with = [&](const void* vectors, long long r, auto&& f) {
+    const uint16_t* vector = static_cast<const uint16_t*>(vectors) + r * p.n;
 #pragma unroll
     for (int i = 0; i < CNT; ++i) {
       float a[8];
-      unpack8<BF16>(team.load_off(vector, t, end, i), a);
+      unpack8<BF16>(team.template load_off<false>(vector, i), a);
       by_pairs<8>(&v[i * 8], [&](uint64_t x, int j) { return f(x, pack2(a[j], a[j + 1])); });
     }
   };
@@ -96,10 +95,10 @@ __global__ void __launch_bounds__(kTeamBlock<THREADS>) residual_norm_kernel(cons
   if (p.post != kNormNone) {
     clear_rest();
     normalize_row(team, v, p.post, inv_n, p.eps, 0);
-    if (p.post_gamma) with(p.post_gamma, 0, p.rows, times);
-    if (p.post_beta) with(p.post_beta, 0, p.rows, plus);
+    if (p.post_gamma) with(p.post_gamma, 0, times);
+    if (p.post_beta) with(p.post_beta, 0, plus);
   }
-  if (p.gate) with(p.gate, row / p.gate_part, p.gate_part, times);
+  if (p.gate) with(p.gate, row / p.gate_part, times);
   if (p.residual != nullptr) {
     const uint64_t scale = pack2(p.residual_scale, p.residual_scale);
 #pragma unroll
@@ -115,8 +114,8 @@ __global__ void __launch_bounds__(kTeamBlock<THREADS>) residual_norm_kernel(cons
   }
   clear_rest();
   normalize_row(team, v, p.norm, inv_n, p.eps, 2);
-  if (p.gamma) with(p.gamma, row / p.gamma_part, p.gamma_part, times);
-  if (p.beta) with(p.beta, row / p.beta_part, p.beta_part, plus);
+  if (p.gamma) with(p.gamma, row / p.gamma_part, times);
+  if (p.beta) with(p.beta, row / p.beta_part, plus);
   if constexpr (QUANTIZE) {
     clear_rest();
     uint32_t most = 0;

@@ -30,8 +30,7 @@ constexpr int kTeamWarpsPerBlock = 8;  // rows of a block where a warp takes a r
 template <int THREADS>
 constexpr int kTeamBlock = THREADS == 32 ? 32 * kTeamWarpsPerBlock : THREADS;
 
-// Eight elements of a piece that reaches over an end of the tensor's memory [lo, hi). Two pieces of a launch do; inlined at every load it
-// filled the instruction cache.
+// Eight elements of a unit that reaches over an end of the memory [lo, hi). (Inlined at every load it filled the instruction cache.)
 static __device__ __noinline__ uint4 load_elements(const uint16_t* at, const uint16_t* lo, const uint16_t* hi) {
   uint32_t e[8];
 #pragma unroll
@@ -96,28 +95,27 @@ struct RowTeam {
     return v;
   }
 
-  // Eight elements on 16 bytes, in one piece unless they reach over an end of the tensor's memory [lo, hi).
-  template <bool STREAM>
-  static __device__ __forceinline__ uint4 piece(const uint16_t* at, const uint16_t* lo, const uint16_t* hi) {
-    if (ALIGNED || (at >= lo && at + 8 <= hi))
-      return STREAM ? ld_stream(reinterpret_cast<const uint4*>(at)) : *reinterpret_cast<const uint4*>(at);
+  // Unit i of row r of `rows` whose memory starts at `lo` and ends at `hi`. What is not the row's holds anything (clear_rest): a unit
+  // that reaches over the row's ends takes its neighbours' elements along.
+  __device__ __forceinline__ uint4 load(const uint16_t* row, bool inner, const uint16_t* lo, const uint16_t* hi, int i) const {
+    if (!has(i)) return make_uint4(0, 0, 0, 0);
+    const uint16_t* at = row - skew + unit(i) * 8;
+    if (ALIGNED || inner || whole(i)) return ld_stream(reinterpret_cast<const uint4*>(at));
     return load_elements(at, lo, hi);
-  }
-  // Unit i of a row of 16-bit elements in a tensor [lo, hi). What is not the row's holds anything (clear_rest).
-  template <bool STREAM>
-  __device__ __forceinline__ uint4 load(const uint16_t* row, const uint16_t* lo, const uint16_t* hi, int i) const {
-    return has(i) ? piece<STREAM>(row - skew + unit(i) * 8, lo, hi) : make_uint4(0, 0, 0, 0);
   }
   // The same elements of a row that may lie at another place of 16 bytes than the team's: the two pieces that hold them, shifted by
   // words and by half a word.
-  __device__ __forceinline__ uint4 load_off(const uint16_t* row, const uint16_t* lo, const uint16_t* hi, int i) const {
-    if (ALIGNED) return load<false>(row, lo, hi, i);
+  template <bool STREAM>
+  __device__ __forceinline__ uint4 load_off(const uint16_t* row, int i) const {
     if (!has(i)) return make_uint4(0, 0, 0, 0);
+    auto fetch = [](const uint16_t* at) {
+      return STREAM ? ld_stream(reinterpret_cast<const uint4*>(at)) : *reinterpret_cast<const uint4*>(at);
+    };
     const uint16_t* at = row + first(i);
+    if (ALIGNED) return fetch(at);
+    if (first(i) < 8 || first(i) + 16 > n) return load_elements(at, row, row + n);
     const int off = static_cast<int>(reinterpret_cast<uintptr_t>(at) >> 1) & 7;
-    const uint4 a = piece<false>(at - off, lo, hi);
-    if (off == 0) return a;
-    const uint4 b = piece<false>(at - off + 8, lo, hi);
+    const uint4 a = fetch(at - off), b = fetch(at - off + 8);
     uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     if (off & 4) {
 #pragma unroll
@@ -266,12 +264,12 @@ struct TeamShape {
 };
 inline TeamShape team_shape(long long rows, long long n, bool aligned, int sms) {
   const long long units = aligned ? n / 8 : (n + 14) / 8;
-  if (units > (aligned ? 4 : 2) * kTeamMaxThreads) return TeamShape{0, kTeamMaxThreads, aligned};
+  if (units > (aligned ? 4 : 3) * kTeamMaxThreads) return TeamShape{0, kTeamMaxThreads, aligned};
   // A few rows are a matter of latency: a unit a thread. Many are one of bytes in flight: up to four.
-  // (Skewed rows take registers: two.)
-  const long long per = rows <= 2ll * sms && units <= kTeamMaxThreads ? 1 : aligned ? 4 : 2;
+  const long long per = rows <= 2ll * sms && units <= kTeamMaxThreads ? 1 : 4;
   int threads = 32;
   while (threads * per < units) threads *= 2;
+  if (!aligned && threads * 3 < units) threads *= 2;  // (skewed rows take registers)
   const int cnt = static_cast<int>((units + threads - 1) / threads);
   return TeamShape{cnt, threads, aligned};
 }
@@ -296,7 +294,7 @@ inline void for_team_shape(const TeamShape& t, F&& launch) {
     return launch(std::integral_constant<int, CNT>{}, std::integral_constant<int, THREADS>{}, std::integral_constant<bool, ALIGNED>{});
 #define B200AIT_TEAMS(THREADS)                                                                                   \
   B200AIT_TEAM(1, THREADS, true) B200AIT_TEAM(2, THREADS, true) B200AIT_TEAM(3, THREADS, true) B200AIT_TEAM(4, THREADS, true) \
-  B200AIT_TEAM(1, THREADS, false) B200AIT_TEAM(2, THREADS, false)
+  B200AIT_TEAM(1, THREADS, false) B200AIT_TEAM(2, THREADS, false) B200AIT_TEAM(3, THREADS, false)
     B200AIT_TEAMS(32) B200AIT_TEAMS(64) B200AIT_TEAMS(128) B200AIT_TEAMS(256) B200AIT_TEAMS(512) B200AIT_TEAMS(1024)
 #undef B200AIT_TEAMS
 #undef B200AIT_TEAM
