@@ -23,6 +23,7 @@
 #include <mutex>
 #include <vector>
 
+#include "b200ait.h"
 #include "gemm_swapab.cuh"
 
 namespace b200ait {
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(256) gemm_simt_i8_kernel(const int8_t* a, cons
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = row0 + ty + i * 8;
-    if (row < p.M) epilogue_scalar_store_i8<BF16>(p, __int2float_rn(acc[i]) * cs, row, col);
+    if (row < p.M) epilogue_scalar_store_i8<BF16>(p, __int2float_rn(acc[i]) * cs, p.row_scale[row], row, col);
   }
 }
 
@@ -458,6 +459,7 @@ struct GemmArgs {
   long long workspace_bytes = 0;
   int split_k = 0;  // 0 = choose, 1 = off, n = at most n splits
   int* status = nullptr;  // device status word to use instead of the library's allocated one
+  int i8_x = 0;  // with i8, for as many rows as rowdot_i8_takes: `a` holds 16-bit elements of this type, quantised on the way
   int i8 = 0;  // a and b are signed 8-bit integers with a scale per row each (dtype is the result's and the residuals')
   const float *row_scale = nullptr, *col_scale = nullptr;
 };
@@ -683,10 +685,15 @@ void gemm_run(const GemmArgs& g_in) {
   p.partial = nullptr;
 
   // (8-bit operands of any K: boxes end in zeros past it, and the copy needs no more than the pitch and the address)
-  const bool tma_ok = g.i8 ? g.lda % 16 == 0 && g.ldb % 16 == 0 && aligned16(g.a) && aligned16(g.b)
+  const bool tma_w_i8 = g.ldb % 16 == 0 && aligned16(g.b);
+  const bool tma_ok = g.i8 ? g.lda % 16 == 0 && aligned16(g.a) && tma_w_i8
                            : (g.k % 8 == 0) && (g.lda % 8 == 0) && (g.ldb % 8 == 0) && aligned16(g.a) && aligned16(g.b) &&
                                  (g.a_bs % 8 == 0) && (g.b_bs % 8 == 0) && g.batch < 65536 * 32;
   B200AIT_REQUIRE(tma_ok || g.num_out == 1, "gemm: several output buffers need TMA-addressable operands");
+  if (g.i8 && tma_w_i8 && g.tile_n == 0 && rowdot_i8_takes(g.m, g.k)) {
+    run_rowdot_i8(g.a, g.i8_x, g.b, p, bf16, g.stream);
+    return;
+  }
   // M <= 4, deep K, the caller left tile width and split-K to the library: stream W once on the CUDA cores
   const long long rowdot_smem = (g.m <= 1 ? 1 : g.m <= 2 ? 2 : 4) * g.k * 2;
   if (tma_ok && !g.i8 && g.batch == 1 && !g.b_mn && g.num_out == 1 && g.tile_n == 0 && g.split_k == 0 &&
@@ -901,21 +908,68 @@ B200AIT_EXPORT int b200ait_gemm_rcr(const void* a, const void* b, const void* bi
   });
 }
 
+static void check_i8(int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb, int64_t ldc, int64_t ldd, int epilogue) {
+  // sums of K products of at most 2^14 each stay below 2^31
+  B200AIT_REQUIRE(k < (1 << 17), "gemm: 8-bit operands take up to 131071 columns");
+  if (m <= 0 || n <= 0) return;
+  B200AIT_REQUIRE(k != 0, "gemm: 8-bit operands have no columns");
+  B200AIT_REQUIRE(k < 0 || (lda >= k && ldb >= k && ldc >= n), "gemm: a row pitch is shorter than the row");
+  const bool residual = epi_b1(epilogue) != kBinaryNone || epi_b2(epilogue) != kBinaryNone;
+  B200AIT_REQUIRE(!residual || ldd >= n, "gemm: a row pitch is shorter than the row");
+}
+static void check_scale(const float* scale) {
+  B200AIT_REQUIRE(scale != nullptr, "gemm: 8-bit operands need the scales of their rows");
+  B200AIT_REQUIRE((reinterpret_cast<uintptr_t>(scale) & 3u) == 0, "gemm: a pointer is not aligned to its type");
+}
+
 // gemm_rcr of signed 8-bit integers: c = epilogue(sum_k a[m, k] b[n, k] * a_scale[m] * b_scale[n] + bias, d0, d1).
 B200AIT_EXPORT int b200ait_gemm_rcr_i8(const void* a, const float* a_scale, const void* b, const float* b_scale,
                                        const void* bias, const void* d0, const void* d1, void* c, int64_t m, int64_t n,
                                        int64_t k, int64_t lda, int64_t ldb, int64_t ldc, int64_t ldd, int epilogue, int dtype,
                                        int tile_n, cudaStream_t stream) {
   return guarded("b200ait_gemm_rcr_i8", [&] {
-    // sums of K products of at most 2^14 each stay below 2^31
-    B200AIT_REQUIRE(k < (1 << 17), "gemm: 8-bit operands take up to 131071 columns");
-    B200AIT_REQUIRE(m <= 0 || n <= 0 || k != 0, "gemm: 8-bit operands have no columns");
-    B200AIT_REQUIRE(m <= 0 || n <= 0 || k <= 0 || (lda >= k && ldb >= k && ldc >= n), "gemm: a row pitch is shorter than the row");
-    const int b1 = epi_b1(epilogue), b2 = epi_b2(epilogue);
-    B200AIT_REQUIRE((b1 == kBinaryNone && b2 == kBinaryNone) || ldd >= n, "gemm: a row pitch is shorter than the row");
+    check_i8(m, n, k, lda, ldb, ldc, ldd, epilogue);
     GemmArgs g{a, b, bias, d0, d1, c, 1, m, n, k, lda, ldb, ldc, ldd, 0, 0, 0, 0, epilogue, dtype, 1.f, 0, 1, 1, 1, tile_n, stream};
-    if (m > 0 && n > 0 && k > 0) B200AIT_REQUIRE(a_scale && b_scale, "gemm: 8-bit operands need the scales of their rows");
+    if (m > 0 && n > 0) check_scale(a_scale), check_scale(b_scale);
     g.i8 = 1, g.row_scale = a_scale, g.col_scale = b_scale;
+    gemm_run(g);
+  });
+}
+
+// The same with its left operand in 16 bits, quantised on the way (quantize.cu): by the product's own kernel for a few rows, else
+// into `scratch`.
+static bool quantizes_by_itself(int64_t m, int64_t k, int64_t ldb, const void* b, int tile_n) {
+  return tile_n == 0 && ldb % 16 == 0 && aligned16(b) && rowdot_i8_takes(m, k);
+}
+static int64_t i8_pitch(int64_t k) { return (k + 15) / 16 * 16; }
+B200AIT_EXPORT int b200ait_gemm_rcr_i8_x16_scratch_bytes(int64_t m, int64_t k, int64_t* bytes_out) {
+  return guarded("b200ait_gemm_rcr_i8_x16_scratch_bytes", [&] {
+    B200AIT_REQUIRE(bytes_out, "bytes_out is null");
+    *bytes_out = m > 0 && k > 0 ? m * i8_pitch(k) + m * 4 : 0;
+  });
+}
+B200AIT_EXPORT int b200ait_gemm_rcr_i8_x16(const void* x, int x_dtype, const void* b, const float* b_scale, const void* bias,
+                                           const void* d0, const void* d1, void* c, int64_t m, int64_t n, int64_t k, int64_t ldx,
+                                           int64_t ldb, int64_t ldc, int64_t ldd, int epilogue, int dtype, int tile_n, void* scratch,
+                                           int64_t scratch_bytes, cudaStream_t stream) {
+  return guarded("b200ait_gemm_rcr_i8_x16", [&] {
+    B200AIT_REQUIRE(x_dtype == kDTypeHalf || x_dtype == kDTypeBFloat16, "gemm: x must be float16 or bfloat16");
+    check_i8(m, n, k, ldx, ldb, ldc, ldd, epilogue);
+    if (m <= 0 || n <= 0) B200AIT_REQUIRE(m >= 0 && n >= 0, "gemm: negative dimension");
+    if (m == 0 || n == 0) return;
+    check_scale(b_scale);
+    B200AIT_REQUIRE(x && (reinterpret_cast<uintptr_t>(x) & 1u) == 0, "gemm: x is null or not aligned to its type");
+    GemmArgs g{x, b, bias, d0, d1, c, 1, m, n, k, ldx, ldb, ldc, ldd, 0, 0, 0, 0, epilogue, dtype, 1.f, 0, 1, 1, 1, tile_n, stream};
+    g.i8 = 1, g.col_scale = b_scale;
+    if (quantizes_by_itself(m, k, ldb, b, tile_n)) {
+      g.i8_x = x_dtype;
+    } else {
+      const int64_t pitch = i8_pitch(k);
+      B200AIT_REQUIRE(scratch && aligned16(scratch) && scratch_bytes >= m * pitch + m * 4, "gemm: the scratch for quantised rows is missing or too small");
+      float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + m * pitch);
+      if (b200ait_quantize_rows(scratch, scale, x, m, k, ldx, pitch, 0, 0, x_dtype, stream) != 0) throw Error(last_error());
+      g.a = scratch, g.lda = pitch, g.row_scale = scale;
+    }
     gemm_run(g);
   });
 }

@@ -252,10 +252,9 @@ __device__ __forceinline__ void epilogue_scalar_store(const GemmParams& p, float
   if (p.bias) v += Elem16<BF16>::to_float(static_cast<const typename Elem16<BF16>::T*>(p.bias)[col]);
   epilogue_scalar_rest<BF16>(p, v, b, row, col);
 }
-// The same on a sum of 8-bit products times its column's scale, rounded as the tile kernels round.
+// The same on a sum of 8-bit products times its column's scale, with its row's scale, rounded as the tile kernels round.
 template <bool BF16>
-__device__ __forceinline__ void epilogue_scalar_store_i8(const GemmParams& p, float scaled, int row, int col) {
-  const float rs = p.row_scale[row];
+__device__ __forceinline__ void epilogue_scalar_store_i8(const GemmParams& p, float scaled, float rs, int row, int col) {
   const float v = p.bias ? __fmaf_rn(scaled, rs, Elem16<BF16>::to_float(static_cast<const typename Elem16<BF16>::T*>(p.bias)[col]))
                          : scaled * rs;
   epilogue_scalar_rest<BF16, true>(p, v, 0, row, col);
@@ -1020,6 +1019,10 @@ void launch_tc_i8<false>(int, const CUtensorMap&, const CUtensorMap&, const OutM
 template <>
 void launch_tc_i8<true>(int, const CUtensorMap&, const CUtensorMap&, const OutMaps&, const CUtensorMap&, const GemmParams&, int,
                         cudaStream_t);
+
+// One to four rows against 8-bit rows of W that start on 16 bytes; defined in gemm_rowdot_i8.cu.
+bool rowdot_i8_takes(long long m, long long k);
+void run_rowdot_i8(const void* x, int x_type, const void* w, const GemmParams& p, bool bf16, cudaStream_t stream);
 
 #define B200AIT_DEFINE_LAUNCH_TC_WIDTH(BN_)                                                                    \
   template <>                                                                                                  \

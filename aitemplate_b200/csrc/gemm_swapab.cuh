@@ -475,7 +475,7 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_const
             for (int e = 0; e < 8; ++e)
               if (col0 + e < p.N) {
                 if constexpr (I8) {
-                  epilogue_scalar_store_i8<BF16>(p, src[e], out_row0 + j, col0 + e);
+                  epilogue_scalar_store_i8<BF16>(p, src[e], row_factor(out_row0 + j), out_row0 + j, col0 + e);
                 } else {
                   epilogue_scalar_store<BF16>(p, src[e], 0, out_row0 + j, col0 + e);
                 }

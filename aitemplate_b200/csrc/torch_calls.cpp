@@ -45,6 +45,7 @@ struct Library {
   decltype(&b200ait_gemm_rcr_i8) gemm_rcr_i8;
   decltype(&b200ait_quantize_rows) quantize_rows;
   decltype(&b200ait_residual_norm) residual_norm;
+  decltype(&b200ait_gemm_rcr_i8_x16) gemm_rcr_i8_x16;
 } lib;
 PyTypeObject* parameter_type = nullptr;  // torch.nn.Parameter
 
@@ -455,8 +456,8 @@ PyObject* gemm_rcr_i8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (x->dim() < 1 || w->dim() != 2 || x->numel() == 0 || w->numel() == 0 || w->size(1) != x->size(-1) ||
         w->scalar_type() != at::kChar || !on_current_device({x, w, w_scale, x_scale, bias, d0, d1}))
       return unhandled();
-    const int64_t n = w->size(0), k = w->size(1), m = x->numel() / k, ldb = row_pitch(*w);
-    int64_t lda = row_pitch(*x);
+    const int64_t n = w->size(0), k = w->size(1), m = x->numel() / k;
+    int64_t lda = row_pitch(*x), ldb = row_pitch(*w);
     if (lda < 0 || ldb < 0) return unhandled();
     const bool has_d0 = ((epilogue >> 4) & 3) != 0, has_d1 = ((epilogue >> 6) & 3) != 0;
     if (has_d0 != (d0 != nullptr) || has_d1 != (d1 != nullptr)) return unhandled();
@@ -475,30 +476,33 @@ PyObject* gemm_rcr_i8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (bias != nullptr && (bias->scalar_type() != type || bias->dim() != 1 || bias->size(0) != n)) return unhandled();
     if (w_scale->scalar_type() != at::kFloat || w_scale->dim() != 1 || w_scale->size(0) != n) return unhandled();
     const b200ait_stream_t stream = current_stream();
-    at::Tensor q, scale;
+    if (n == 1) ldb = padded(k);  // (a single row has any pitch)
     if (x->scalar_type() == at::kChar) {
       if (!x_scale || x_scale->scalar_type() != at::kFloat ||
           x_scale->sizes() != x->sizes().slice(0, static_cast<size_t>(x->dim() - 1)))
         return unhandled();
-    } else {
-      if (x_scale || dtype_code(*x) == 0) return unhandled();
-      q = at::empty({m, padded(k)}, x->options().dtype(at::kChar)), scale = row_scales(*x);
+      if (m == 1) lda = padded(k);
+      at::Tensor y = at::empty(shape, x->options().dtype(type));
       if (unlocked([&] {
-            return lib.quantize_rows(q.data_ptr(), static_cast<float*>(scale.data_ptr()), pointer(x), m, k, lda, padded(k), 0, 0,
-                                     dtype_code(*x), stream);
+            return lib.gemm_rcr_i8(pointer(x), static_cast<const float*>(pointer(x_scale)), pointer(w),
+                                   static_cast<const float*>(pointer(w_scale)), pointer(bias), pointer(d0), pointer(d1), y.data_ptr(), m,
+                                   n, k, lda, ldb, n, n, static_cast<int>(epilogue), dtype_code(y), static_cast<int>(tile_n), stream);
           }))
-        return failed("b200ait_quantize_rows");
-      lda = padded(k);
+        return failed("b200ait_gemm_rcr_i8");
+      return THPVariable_Wrap(std::move(y));
     }
-    at::Tensor y = at::empty(shape, x->options().dtype(type));
-    const void* a = q.defined() ? q.data_ptr() : pointer(x);
-    const float* a_scale = static_cast<const float*>(scale.defined() ? scale.data_ptr() : pointer(x_scale));
+    if (x_scale || dtype_code(*x) == 0) return unhandled();
+    at::Tensor y = at::empty(shape, x->options().dtype(type)), scratch;
+    // (a few rows need none, but for W off 16 bytes)
+    const int64_t bytes = m <= 4 && tile_n == 0 && ldb % 16 == 0 && k <= 32768 ? 0 : m * padded(k) + m * 4;
+    if (bytes != 0) scratch = at::empty({bytes}, x->options().dtype(at::kByte));
     if (unlocked([&] {
-          return lib.gemm_rcr_i8(a, a_scale, pointer(w), static_cast<const float*>(pointer(w_scale)), pointer(bias), pointer(d0),
-                                 pointer(d1), y.data_ptr(), m, n, k, m == 1 ? padded(k) : lda, n == 1 ? padded(k) : ldb, n, n,
-                                 static_cast<int>(epilogue), dtype_code(y), static_cast<int>(tile_n), stream);
+          return lib.gemm_rcr_i8_x16(pointer(x), dtype_code(*x), pointer(w), static_cast<const float*>(pointer(w_scale)), pointer(bias),
+                                     pointer(d0), pointer(d1), y.data_ptr(), m, n, k, lda, ldb, n, n, static_cast<int>(epilogue),
+                                     dtype_code(y), static_cast<int>(tile_n), scratch.defined() ? scratch.data_ptr() : nullptr, bytes,
+                                     stream);
         }))
-      return failed("b200ait_gemm_rcr_i8");
+      return unhandled();  // (the Python code gives it scratch in any case)
     return THPVariable_Wrap(std::move(y));
   });
 }

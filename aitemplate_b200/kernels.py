@@ -490,9 +490,11 @@ def gemm_rcr_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale
     elif x_scale is not None:
         raise ValueError(f"{what}: x_scale goes with an int8 x, got {x.dtype}")
     else:
-        x, x_scale = quantize_rows(x)
+        x_code = _dtype_code(x)
     lead = x.shape[:-1]
     for name, t, shape in (("w_scale", w_scale, (n,)), ("x_scale", x_scale, tuple(lead))):
+        if t is None:
+            continue
         if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
             raise ValueError(f"{what}: {name} must be a contiguous float32 tensor of shape {shape}")
     if epilogue not in EPILOGUES:
@@ -510,12 +512,20 @@ def gemm_rcr_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale
         if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
             raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {shape}")
     lda, ldb = _row_pitch(what, "x", x), _row_pitch(what, "w", w)
+    ldb = _padded(k) if n == 1 else ldb  # (a single row has any pitch)
     m = math.prod(lead)
     y = torch.empty(out_shape, dtype=dtype, device=x.device)
-    code = _lib.load().b200ait_gemm_rcr_i8(_ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(bias), _ptr(d0), _ptr(d1), _ptr(y),
-                                           m, n, k, _padded(k) if m == 1 else lda, _padded(k) if n == 1 else ldb, n, n,
-                                           epilogue_code(epilogue), _DTYPE_CODE[dtype], tile_n, _stream())
-    _lib.check(code, "b200ait_gemm_rcr_i8")
+    rest = (_ptr(bias), _ptr(d0), _ptr(d1), _ptr(y), m, n, k)
+    if x_scale is not None:
+        code = _lib.load().b200ait_gemm_rcr_i8(_ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), *rest, _padded(k) if m == 1 else lda, ldb,
+                                               n, n, epilogue_code(epilogue), _DTYPE_CODE[dtype], tile_n, _stream())
+        _lib.check(code, "b200ait_gemm_rcr_i8")
+        return y
+    scratch_bytes = m * _padded(k) + m * 4
+    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=x.device)
+    code = _lib.load().b200ait_gemm_rcr_i8_x16(_ptr(x), x_code, _ptr(w), _ptr(w_scale), *rest, lda, ldb, n, n, epilogue_code(epilogue),
+                                               _DTYPE_CODE[dtype], tile_n, _ptr(scratch), scratch_bytes, _stream())
+    _lib.check(code, "b200ait_gemm_rcr_i8_x16")
     return y
 
 

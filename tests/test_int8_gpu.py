@@ -556,13 +556,74 @@ def test_captured_and_on_another_stream():
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
 
 
-def test_16_bit_rows_are_quantised_on_the_way():
-    for m, k in ((1, 512), (7, 300), (200, 768)):
-        x = torch.randn(m, k, generator=_gen(m), device="cuda").to(torch.float16)
-        w, ws = _weights(136, k, 2)
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 40, 200])
+@pytest.mark.parametrize("k", [1, 8, 300, 512, 1023, 1024, 2041, 4096, 10000])
+def test_16_bit_rows_are_quantised_on_the_way(m, k):
+    """In one call or two, by the product's own kernel or into scratch: the same result."""
+    for dtype, out in ((torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.bfloat16)):
+        x = torch.randn(m, k, generator=_gen(m), device="cuda").to(dtype)
+        x[m // 2, :k // 2] *= 40
+        w, ws = _weights(139, k, 2)
+        b, d0 = (torch.randn(*s, generator=_gen(k), device="cuda").to(out) for s in ((139,), (m, 139)))
         q, scale = kernels.quantize_rows(x)
-        assert torch.equal(kernels.gemm_rcr_i8(x, w, ws), kernels.gemm_rcr_i8(q, w, ws, scale))
-        assert kernels.gemm_rcr_i8(x, w, ws, dtype=torch.bfloat16).dtype == torch.bfloat16
+        want = kernels.gemm_rcr_i8(q, w, ws, scale, bias=b, d0=d0, epilogue="add", dtype=out)
+        ref, off = _product64(q, w, scale, ws, b, d0, None, "add")
+        _close(want, ref, off, out)
+        for form in (x, _at(x, 3), torch.cat([x, x, x], 1)[:, k:2 * k]):  # rows on and off 16 bytes, and apart
+            assert torch.equal(kernels.gemm_rcr_i8(form, w, ws, bias=b, d0=d0, epilogue="add", dtype=out), want)
+        assert torch.equal(kernels.gemm_rcr_i8(x, w.contiguous(), ws, bias=b, d0=d0, epilogue="add", dtype=out), want)
+    x[0, 0] = math.inf
+    y = kernels.gemm_rcr_i8(x, w, ws)
+    assert bool(torch.isnan(y[0]).all()) and not torch.isnan(y[1:]).any()
+
+
+def test_a_few_rows_of_any_place_and_shape():
+    """One to four rows against many, few and no whole turns of columns, W with rows apart and its last row at the end of its memory."""
+    for m in (1, 2, 3, 4):
+        for n, k in ((1, 64), (2, 5000), (37, 512), (148, 513), (593, 1024), (3001, 1040), (4097, 528), (600, 2064), (9000, 256), (300, 20000)):
+            _check_product(m, n, k, DTYPES[n % 2], ("", "add", "mul_add", "gelu")[(m + n) % 4], True, n, pitch_w=(k + 31) // 16 * 16)
+
+
+def test_the_native_path_and_the_python_code_agree(monkeypatch):
+    from aitemplate_b200 import _lib
+
+    class Absent:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    class Recorder:
+        def __init__(self):
+            self.module, self.served = _lib.load_calls(), []
+
+        def __getattr__(self, name):
+            def call(*args):
+                y = getattr(self.module, name)(*args)
+                self.served.append(y is not None)
+                return y
+            return call
+
+    x, w, ws, xs, b, d0, _ = _problem(6, 40, 72, torch.float16, "add", True, 1, 80, 96)
+    h = torch.randn(2, 3, 72, generator=_gen(1), device="cuda").to(torch.bfloat16)
+    n, o = _norm_operands(6, 72, torch.float16, 1, 3, "rms", "layer")
+    calls = [
+        lambda: kernels.gemm_rcr_i8(x, w, ws, xs, bias=b, d0=d0, epilogue="add"), lambda: kernels.gemm_rcr_i8(x, w, ws, xs),
+        lambda: kernels.gemm_rcr_i8(x, w, ws, xs, dtype=torch.bfloat16, tile_n=64), lambda: kernels.gemm_rcr_i8(h, w, ws),
+        lambda: kernels.gemm_rcr_i8(h, w, ws, dtype=torch.float16), lambda: kernels.gemm_rcr_i8(h[0, :1], w, ws, bias=b.bfloat16()),
+        lambda: kernels.gemm_rcr_i8(h[:, 1], w, ws), lambda: kernels.quantize_rows(h), lambda: kernels.quantize_rows(h[:, 1], "swish", True),
+        lambda: kernels.quantize_rows(torch.nn.Parameter(h[0])), lambda: kernels.residual_norm(n, **o),
+        lambda: kernels.residual_norm(n, quantize=True, **o), lambda: kernels.residual_norm(h, norm="rms"),
+    ]
+    for call in calls:
+        with monkeypatch.context() as c:
+            recorder = Recorder()
+            c.setattr(kernels, "_calls", recorder)
+            native = call()
+            assert recorder.served == [True]
+        with monkeypatch.context() as c:
+            c.setattr(kernels, "_calls", Absent())
+            python = call()
+        for p, q in zip(*((r,) if torch.is_tensor(r) else r for r in (native, python))):
+            assert p.shape == q.shape and p.dtype == q.dtype and p.stride() == q.stride() and torch.equal(p, q)
 
 
 def test_refusals():
