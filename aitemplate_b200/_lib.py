@@ -53,7 +53,7 @@ def _signatures():
         "b200ait_gemm_rcr_i8_x16": (
             c_int, [c_void_p, c_int] + [c_void_p] * 6 + [c_int64] * 7 + [c_int] * 3 + [c_void_p, c_int64, c_void_p],
         ),
-        "b200ait_gemm_rcr_i8_x16_scratch_bytes": (c_int, [c_int64, c_int64, I64P]),
+        "b200ait_gemm_rcr_i8_x16_scratch_bytes": (c_int, [c_void_p] + [c_int64] * 4 + [c_int, I64P]),
         "b200ait_quantize_rows": (c_int, [c_void_p] * 3 + [c_int64] * 4 + [c_int] * 3 + [c_void_p]),
         "b200ait_residual_norm": (
             c_int, [c_void_p] * 10 + [c_int64] * 6 + [c_int, c_int, c_float, c_float, c_int, c_void_p],
@@ -149,7 +149,8 @@ def load() -> ctypes.CDLL:
 _CALLED = ["b200ait_gemm_rcr", "b200ait_gemm_rrr", "b200ait_gemm_rcr_scratch_bytes", "b200ait_mem_eff_attention",
            "b200ait_flash_attention", "b200ait_layernorm", "b200ait_softmax", "b200ait_concatenate", "b200ait_split",
            "b200ait_permute", "b200ait_last_error", "AITemplateModelContainerRun", "b200ait_gemm_rcr_i8",
-           "b200ait_quantize_rows", "b200ait_residual_norm", "b200ait_gemm_rcr_i8_x16"]
+           "b200ait_quantize_rows", "b200ait_residual_norm", "b200ait_gemm_rcr_i8_x16",
+           "b200ait_gemm_rcr_i8_x16_scratch_bytes"]
 _calls = None
 
 

@@ -346,8 +346,8 @@ static const std::vector<SwapKernel>& swap_kernels() {
 //
 // From 64 rows on: by the estimates of rules.h, X in groups that are as small as it takes to fill one wave. The tile
 // kernels' are the firmer ones where both are close.
-static const SwapKernel* plan_swapab(const GemmProblem& g, int tile_width, bool bf16) {
-  if (g.n < 128 || g.m < 5 || g.k < 256) return nullptr;
+static const SwapKernel* plan_swapab(const GemmProblem& g, int tile_width, bool bf16, int from_rows) {
+  if (g.n < 128 || g.m < from_rows || g.k < 256) return nullptr;
   const long long slabs = (g.n + 127) / 128, kb_total = (g.k + kBK - 1) / kBK;
   const auto& table = swap_kernels();
   const SwapKernel* best = nullptr;
@@ -459,7 +459,7 @@ struct GemmArgs {
   long long workspace_bytes = 0;
   int split_k = 0;  // 0 = choose, 1 = off, n = at most n splits
   int* status = nullptr;  // device status word to use instead of the library's allocated one
-  int i8_x = 0;  // with i8, for as many rows as rowdot_i8_takes: `a` holds 16-bit elements of this type, quantised on the way
+  int i8_x = 0;  // with i8, where gemm_i8_rowdot says so: `a` holds 16-bit elements of this type, quantised on the way
   int i8 = 0;  // a and b are signed 8-bit integers with a scale per row each (dtype is the result's and the residuals')
   const float *row_scale = nullptr, *col_scale = nullptr;
 };
@@ -496,14 +496,14 @@ struct GemmPlan {
 };
 // The estimates of one problem take about half a microsecond of host time, which a call of a few microseconds would pay every
 // time: each thread keeps the plans of the problem sizes it saw last (by their sizes alone; 64 of them).
-static GemmPlan plan_gemm(const GemmProblem& g, bool bf16, bool streams) {
+static GemmPlan plan_gemm(const GemmProblem& g, bool bf16, bool streams, int from_rows) {
   struct Slot {
     GemmProblem g;
     int sms, flags;
     GemmPlan plan;
   };
   thread_local Slot slots[64] = {};
-  const int sms = sm_count(), flags = 1 | (bf16 ? 2 : 0) | (streams ? 4 : 0);
+  const int sms = sm_count(), flags = 1 | (bf16 ? 2 : 0) | (streams ? 4 : 0) | from_rows << 3;
   uint64_t h = static_cast<uint64_t>(g.batch);
   for (const long long v : {g.m, g.n, g.k, g.pitch, static_cast<long long>(g.epilogue * 16 + g.swap_epilogue * 4 + g.generic * 64 + g.pairs * 128 + flags * 256)})
     h = (h ^ static_cast<uint64_t>(v)) * 0x9e3779b97f4a7c15ull;
@@ -513,7 +513,7 @@ static GemmPlan plan_gemm(const GemmProblem& g, bool bf16, bool streams) {
       s.g.pairs == g.pairs)
     return s.plan;
   GemmPlan plan{choose_tile_n(g), nullptr};
-  if (streams) plan.swap = plan_swapab(g, plan.tile_n, bf16);
+  if (streams) plan.swap = plan_swapab(g, plan.tile_n, bf16, from_rows);
   s = Slot{g, sms, flags, plan};
   return plan;
 }
@@ -690,7 +690,7 @@ void gemm_run(const GemmArgs& g_in) {
                            : (g.k % 8 == 0) && (g.lda % 8 == 0) && (g.ldb % 8 == 0) && aligned16(g.a) && aligned16(g.b) &&
                                  (g.a_bs % 8 == 0) && (g.b_bs % 8 == 0) && g.batch < 65536 * 32;
   B200AIT_REQUIRE(tma_ok || g.num_out == 1, "gemm: several output buffers need TMA-addressable operands");
-  if (g.i8 && tma_w_i8 && g.tile_n == 0 && rowdot_i8_takes(g.m, g.k)) {
+  if (g.i8 && tma_w_i8 && g.tile_n == 0 && gemm_i8_rowdot(g.m, g.n, g.k, g.i8_x != 0)) {
     run_rowdot_i8(g.a, g.i8_x, g.b, p, bf16, g.stream);
     return;
   }
@@ -763,7 +763,7 @@ void gemm_run(const GemmArgs& g_in) {
                        (epi_u1(code) == kUnaryIdentity || epi_u1(code) == kUnaryRelu) && p.store_mode == 0;
     problem.swap_epilogue = !plain ? 2 : added ? 1 : 0;
     problem.epilogue = b1 != kBinaryNone ? 1 : epi_u1(code) != kUnaryIdentity && epi_u1(code) != kUnaryRelu ? 2 : 0;
-    if (g.tile_n == 0) planned = plan_gemm(problem, bf16, streams);
+    if (g.tile_n == 0) planned = plan_gemm(problem, bf16, streams, g.i8 ? 1 : 5);
     if (const SwapKernel* sk = planned.swap) {
       const int num_groups = static_cast<int>((g.m + sk->mx - 1) / sk->mx);
       const int num_slabs = static_cast<int>((g.n + 127) / 128);
@@ -938,14 +938,16 @@ B200AIT_EXPORT int b200ait_gemm_rcr_i8(const void* a, const float* a_scale, cons
 
 // The same with its left operand in 16 bits, quantised on the way (quantize.cu): by the product's own kernel for a few rows, else
 // into `scratch`.
-static bool quantizes_by_itself(int64_t m, int64_t k, int64_t ldb, const void* b, int tile_n) {
-  return tile_n == 0 && ldb % 16 == 0 && aligned16(b) && rowdot_i8_takes(m, k);
-}
 static int64_t i8_pitch(int64_t k) { return (k + 15) / 16 * 16; }
-B200AIT_EXPORT int b200ait_gemm_rcr_i8_x16_scratch_bytes(int64_t m, int64_t k, int64_t* bytes_out) {
+static int64_t x16_scratch_bytes(int64_t m, int64_t n, int64_t k, int64_t ldb, const void* b, int tile_n) {
+  if (m <= 0 || n <= 0 || k <= 0 || (tile_n == 0 && ldb % 16 == 0 && aligned16(b) && gemm_i8_rowdot(m, n, k, true))) return 0;
+  return m * i8_pitch(k) + m * 4;
+}
+B200AIT_EXPORT int b200ait_gemm_rcr_i8_x16_scratch_bytes(const void* b, int64_t m, int64_t n, int64_t k, int64_t ldb, int tile_n,
+                                                         int64_t* bytes_out) {
   return guarded("b200ait_gemm_rcr_i8_x16_scratch_bytes", [&] {
     B200AIT_REQUIRE(bytes_out, "bytes_out is null");
-    *bytes_out = m > 0 && k > 0 ? m * i8_pitch(k) + m * 4 : 0;
+    *bytes_out = x16_scratch_bytes(m, n, k, ldb, b, tile_n);
   });
 }
 B200AIT_EXPORT int b200ait_gemm_rcr_i8_x16(const void* x, int x_dtype, const void* b, const float* b_scale, const void* bias,
@@ -961,11 +963,12 @@ B200AIT_EXPORT int b200ait_gemm_rcr_i8_x16(const void* x, int x_dtype, const voi
     B200AIT_REQUIRE(x && (reinterpret_cast<uintptr_t>(x) & 1u) == 0, "gemm: x is null or not aligned to its type");
     GemmArgs g{x, b, bias, d0, d1, c, 1, m, n, k, ldx, ldb, ldc, ldd, 0, 0, 0, 0, epilogue, dtype, 1.f, 0, 1, 1, 1, tile_n, stream};
     g.i8 = 1, g.col_scale = b_scale;
-    if (quantizes_by_itself(m, k, ldb, b, tile_n)) {
+    const int64_t needed = x16_scratch_bytes(m, n, k, ldb, b, tile_n);
+    if (needed == 0) {
       g.i8_x = x_dtype;
     } else {
       const int64_t pitch = i8_pitch(k);
-      B200AIT_REQUIRE(scratch && aligned16(scratch) && scratch_bytes >= m * pitch + m * 4, "gemm: the scratch for quantised rows is missing or too small");
+      B200AIT_REQUIRE(scratch && aligned16(scratch) && scratch_bytes >= needed, "gemm: the scratch for quantised rows is missing or too small");
       float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + m * pitch);
       if (b200ait_quantize_rows(scratch, scale, x, m, k, ldx, pitch, 0, 0, x_dtype, stream) != 0) throw Error(last_error());
       g.a = scratch, g.lda = pitch, g.row_scale = scale;

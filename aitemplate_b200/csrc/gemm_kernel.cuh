@@ -1020,8 +1020,7 @@ template <>
 void launch_tc_i8<true>(int, const CUtensorMap&, const CUtensorMap&, const OutMaps&, const CUtensorMap&, const GemmParams&, int,
                         cudaStream_t);
 
-// One to four rows against 8-bit rows of W that start on 16 bytes; defined in gemm_rowdot_i8.cu.
-bool rowdot_i8_takes(long long m, long long k);
+// A few rows (gemm_i8_rowdot in rules.h) against 8-bit rows of W that start on 16 bytes; defined in gemm_rowdot_i8.cu.
 void run_rowdot_i8(const void* x, int x_type, const void* w, const GemmParams& p, bool bf16, cudaStream_t stream);
 
 #define B200AIT_DEFINE_LAUNCH_TC_WIDTH(BN_)                                                                    \

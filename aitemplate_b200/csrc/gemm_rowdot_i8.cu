@@ -12,7 +12,7 @@
 namespace b200ait {
 
 constexpr int kRowDotI8Threads = 512;
-constexpr int kRowDotI8Smem = 160 * 1024;  // for the rows of X
+constexpr int kRowDotI8Smem = 160 * 1024;  // for the rows of X (gemm_i8_rowdot)
 
 // X to shared memory, `pad` bytes a row, zeros past K
 template <int MR>
@@ -182,10 +182,6 @@ static void launch_rowdot_i8(const void* x, const int8_t* w, const GemmParams& p
   launch_early(kernel, dim3(static_cast<unsigned>(grid)), kRowDotI8Threads, static_cast<size_t>(smem), stream, true, 1, x, w, p);
 }
 
-bool rowdot_i8_takes(long long m, long long k) {
-  return m >= 1 && m <= 4 && (m <= 2 ? m : 4) * ((k + 15) / 16 * 16) <= kRowDotI8Smem;
-}
-
 // x_type: 0 for 8-bit rows with p.row_scale, else the DType of 16-bit ones
 void run_rowdot_i8(const void* x, int x_type, const void* w, const GemmParams& p, bool bf16, cudaStream_t stream) {
   const int8_t* w8 = static_cast<const int8_t*>(w);
@@ -195,8 +191,9 @@ void run_rowdot_i8(const void* x, int x_type, const void* w, const GemmParams& p
 #define B200AIT_ONE(BF, MR, KV, TYPE) \
   case ((BF) * 3 + (TYPE)) * 100 + (MR) * 10 + (KV): return launch_rowdot_i8<(BF) != 0, MR, KV, TYPE>(x, w8, p, stream);
 #define B200AIT_KVS(BF, MR, TYPE) B200AIT_ONE(BF, MR, 1, TYPE) B200AIT_ONE(BF, MR, 2, TYPE) B200AIT_ONE(BF, MR, 4, TYPE) B200AIT_ONE(BF, MR, 8, TYPE)
-#define B200AIT_ROWS(BF, TYPE) B200AIT_KVS(BF, 1, TYPE) B200AIT_KVS(BF, 2, TYPE) B200AIT_KVS(BF, 4, TYPE)
+#define B200AIT_ROWS(BF, TYPE) B200AIT_KVS(BF, 1, TYPE) B200AIT_KVS(BF, 2, TYPE)
     B200AIT_ROWS(0, 0) B200AIT_ROWS(0, 1) B200AIT_ROWS(0, 2) B200AIT_ROWS(1, 0) B200AIT_ROWS(1, 1) B200AIT_ROWS(1, 2)
+    B200AIT_KVS(0, 4, 1) B200AIT_KVS(0, 4, 2) B200AIT_KVS(1, 4, 1) B200AIT_KVS(1, 4, 2)  // (8-bit rows: rules.h sends no more than two)
 #undef B200AIT_ROWS
 #undef B200AIT_KVS
 #undef B200AIT_ONE

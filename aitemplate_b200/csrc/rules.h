@@ -239,6 +239,19 @@ inline bool gemm_may_split(long long m, long long n, long long k) {
   return !(m >= 5 && n >= 128) && !gemm_rowdot_long(m, n, k);
 }
 
+// GEMM of 8-bit integers, a few rows of X: on the CUDA cores (gemm_rowdot_i8.cu) or, from 128 columns and K = 256 on, by the weight-streaming
+// kernel, whose time does not grow with the rows. us, CUDA cores with 1 / 2 / 4 rows and the other: 4096 x 4096 5.5 / 6.4 / 7.7, 5.9;
+// 1024 x 1024 2.1 / 2.7 / 4.0, 3.2; 2048 x 2048 3.0 / 3.5 / 4.4, 4.2; 1024 x 4096 2.9 / 3.4 / 4.3, 4.5; 8192 x 8192 12.8 / 13.4 / 18.2, 12.8;
+// 14336 x 4096 12.0 / 13.2 / 17.7, 11.8; 4096 x 512 2.5 / 3.8 / 6.8, 3.1; 16384 x 1024 5.3 / 5.7 / 9.0, 7.1. With X in 16 bits
+// the other one needs a launch ahead of it to quantise them, which the CUDA cores do on the way: 2 rows 3.9 and 5.7 (2048 x 2048), 6.7 and
+// 7.6 (4096 x 4096), 4 rows 6.1 and 5.7, 9.7 and 7.6, and 3 us less on the host, which sets the pace of calls of this size.
+inline bool gemm_i8_rowdot(long long m, long long n, long long k, bool x16) {
+  constexpr long long kShared = 160 << 10;  // for the rows of X
+  if (m < 1 || m > 4 || (m <= 2 ? m : 4) * ((k + 15) / 16 * 16) > kShared) return false;
+  if (m == 1 || (m == 2 && (x16 || n < 128 || k < 256))) return true;
+  return n * k <= (m == 2 ? 8ll << 20 : 4ll << 20) && (x16 || (m == 2 && k >= 1024));
+}
+
 // May a tile kernel's CTAs become resident before the kernel ahead of it has ended (launch_early)? It saves 0.4 .. 0.8 us (3 .. 25 %
 // of launches under 15 us), but CTAs then take the SMs in the order in which these fall free, so that neighbouring tiles no
 // longer lie on neighbouring SMs: where the CTAs walk several tiles each that costs more than it saves (4096^3 bf16 99 -> 103

@@ -46,6 +46,7 @@ struct Library {
   decltype(&b200ait_quantize_rows) quantize_rows;
   decltype(&b200ait_residual_norm) residual_norm;
   decltype(&b200ait_gemm_rcr_i8_x16) gemm_rcr_i8_x16;
+  decltype(&b200ait_gemm_rcr_i8_x16_scratch_bytes) x16_scratch_bytes;
 } lib;
 PyTypeObject* parameter_type = nullptr;  // torch.nn.Parameter
 
@@ -493,8 +494,8 @@ PyObject* gemm_rcr_i8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     }
     if (x_scale || dtype_code(*x) == 0) return unhandled();
     at::Tensor y = at::empty(shape, x->options().dtype(type)), scratch;
-    // (a few rows need none, but for W off 16 bytes)
-    const int64_t bytes = m <= 4 && tile_n == 0 && ldb % 16 == 0 && k <= 32768 ? 0 : m * padded(k) + m * 4;
+    int64_t bytes = 0;
+    if (lib.x16_scratch_bytes(pointer(w), m, n, k, ldb, static_cast<int>(tile_n), &bytes) != 0) return unhandled();
     if (bytes != 0) scratch = at::empty({bytes}, x->options().dtype(at::kByte));
     if (unlocked([&] {
           return lib.gemm_rcr_i8_x16(pointer(x), dtype_code(*x), pointer(w), static_cast<const float*>(pointer(w_scale)), pointer(bias),
@@ -502,7 +503,7 @@ PyObject* gemm_rcr_i8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                                      dtype_code(y), static_cast<int>(tile_n), scratch.defined() ? scratch.data_ptr() : nullptr, bytes,
                                      stream);
         }))
-      return unhandled();  // (the Python code gives it scratch in any case)
+      return failed("b200ait_gemm_rcr_i8_x16");
     return THPVariable_Wrap(std::move(y));
   });
 }

@@ -521,10 +521,12 @@ def gemm_rcr_i8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale
                                                n, n, epilogue_code(epilogue), _DTYPE_CODE[dtype], tile_n, _stream())
         _lib.check(code, "b200ait_gemm_rcr_i8")
         return y
-    scratch_bytes = m * _padded(k) + m * 4
-    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=x.device)
+    needed = c_int64(0)
+    code = _lib.load().b200ait_gemm_rcr_i8_x16_scratch_bytes(_ptr(w), m, n, k, ldb, tile_n, ctypes.byref(needed))
+    _lib.check(code, "b200ait_gemm_rcr_i8_x16_scratch_bytes")
+    scratch = torch.empty(needed.value, dtype=torch.uint8, device=x.device)
     code = _lib.load().b200ait_gemm_rcr_i8_x16(_ptr(x), x_code, _ptr(w), _ptr(w_scale), *rest, lda, ldb, n, n, epilogue_code(epilogue),
-                                               _DTYPE_CODE[dtype], tile_n, _ptr(scratch), scratch_bytes, _stream())
+                                               _DTYPE_CODE[dtype], tile_n, _ptr(scratch), needed.value, _stream())
     _lib.check(code, "b200ait_gemm_rcr_i8_x16")
     return y
 

@@ -135,14 +135,15 @@ int b200ait_gemm_rcr_i8(const void* a, const float* a_scale, const void* b, cons
                         const void* d0, const void* d1, void* c, int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb,
                         int64_t ldc, int64_t ldd, int epilogue, int dtype, int tile_n, b200ait_stream_t stream);
 
-/* The same with the left operand in 16 bits (x_dtype), quantised on the way as by b200ait_quantize_rows: one to four rows against rows
- * of b that start on 16 bytes (tile_n = 0) by the product's own kernel, others into `scratch` (16-byte aligned, at least the bytes that
- * b200ait_gemm_rcr_i8_x16_scratch_bytes reports for any b). */
+/* The same with the left operand in 16 bits (x_dtype), quantised on the way as by b200ait_quantize_rows: a few rows by the product's
+ * own kernel, others into `scratch` (16-byte aligned), of which b200ait_gemm_rcr_i8_x16_scratch_bytes says how much the call needs
+ * (0: none; of b it reads the address alone). */
 int b200ait_gemm_rcr_i8_x16(const void* x, int x_dtype, const void* b, const float* b_scale, const void* bias, const void* d0,
                             const void* d1, void* c, int64_t m, int64_t n, int64_t k, int64_t ldx, int64_t ldb, int64_t ldc,
                             int64_t ldd, int epilogue, int dtype, int tile_n, void* scratch, int64_t scratch_bytes,
                             b200ait_stream_t stream);
-int b200ait_gemm_rcr_i8_x16_scratch_bytes(int64_t m, int64_t k, int64_t* bytes_out);
+int b200ait_gemm_rcr_i8_x16_scratch_bytes(const void* b, int64_t m, int64_t n, int64_t k, int64_t ldb, int tile_n,
+                                          int64_t* bytes_out);
 
 /* fp16 entry points with the reference's generated signatures. workspace / split_k are accepted
  * and ignored. *c_dim0, *c_dim1 are written.
