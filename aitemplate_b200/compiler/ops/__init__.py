@@ -3,6 +3,7 @@
 from .attention import *  # noqa: F401,F403
 from .common import *  # noqa: F401,F403
 from .gemm_universal import *  # noqa: F401,F403
+from .int8 import *  # noqa: F401,F403
 from .layernorm import *  # noqa: F401,F403
 from .softmax import *  # noqa: F401,F403
 from .tensor import *  # noqa: F401,F403

@@ -63,6 +63,14 @@ int b200ait_split(void* const*, const uint8_t*, const void*, const int64_t*, int
 int b200ait_permute(const void*, void*, const int64_t*, const int64_t*, int64_t, int64_t, cudaStream_t);
 int b200ait_elementwise(void*, const int64_t*, int64_t, const void* const*, const int64_t* const*, int64_t, const int*,
                         const int*, const float*, int64_t, int, cudaStream_t);
+int b200ait_gemm_rcr_i8(const void*, const float*, const void*, const float*, const void*, const void*, const void*, void*, int64_t,
+                        int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int, int, int, cudaStream_t);
+int b200ait_gemm_rcr_i8_x16(const void*, int, const void*, const float*, const void*, const void*, const void*, void*, int64_t, int64_t,
+                            int64_t, int64_t, int64_t, int64_t, int64_t, int, int, int, void*, int64_t, cudaStream_t);
+int b200ait_gemm_rcr_i8_x16_scratch_bytes(const void*, int64_t, int64_t, int64_t, int64_t, int, int64_t*);
+int b200ait_quantize_rows(void*, float*, const void*, int64_t, int64_t, int64_t, int64_t, int, int, int, cudaStream_t);
+int b200ait_residual_norm(void*, void*, float*, const void*, const void*, const void*, const void*, const void*, const void*, const void*,
+                          int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int, int, float, float, int, cudaStream_t);
 int b200ait_device_status(int*);
 }
 
@@ -91,7 +99,7 @@ static size_t dtype_size(int dtype) {
     case 1: case 6: return 2;
     case 2: case 3: return 4;
     case 4: return 8;
-    case 5: return 1;
+    case 5: case 7: return 1;
     default: throw Error("dtype handling is not implemented!");
   }
 }
@@ -309,6 +317,15 @@ class Executor {
       }
     }
     workspace_bytes_ = std::min<int64_t>(workspace_bytes_, 256ll << 20);
+    // gemm_rcr_i8 of 16-bit rows: room for as many quantised ones as the dynamic dims allow (more than any number of rows below needs)
+    for (const OpInfo& op : plan.ops) {
+      if (op.kernel != "gemm_rcr_i8" || op.operands.size() < 3 || op.operands[1] >= 0) continue;
+      const TensorInfo& a = plan.tensors[op.operands[0]];
+      if (a.dims.empty() || !a.dims.back().is_static) continue;
+      int64_t rows = 1;
+      for (size_t i = 0; i + 1 < a.dims.size(); ++i) rows *= a.dims[i].is_static ? a.dims[i].v : plan.dims[a.dims[i].v].hi;
+      workspace_bytes_ = std::max(workspace_bytes_, rows * ((a.dims.back().v + 15) / 16 * 16 + 4));
+    }
     if (workspace_bytes_ > 0) workspace_ = alloc_.Allocate(static_cast<size_t>(workspace_bytes_));
     B200AIT_CUDA_CHECK(cudaEventCreateWithFlags(&run_finished_, cudaEventDisableTiming));
     B200AIT_CUDA_CHECK(cudaStreamCreateWithFlags(&graph_stream_, cudaStreamNonBlocking));
@@ -652,6 +669,70 @@ void Executor::run_one(const OpInfo& op, cudaStream_t stream, bool launch) {
     uint8_t* y = static_cast<uint8_t*>(ptr_of(out0)) + out_off * dtype_size(T[out0].dtype);
     check(b200ait_layernorm(y, ptr_of(x), ptr_of(in(1)), ptr_of(in(2)), m, n, static_cast<float>(op.floats[0]),
                             in_stride, out_stride, T[x].dtype, stream),
+          op);
+    return;
+  }
+  if (op.kernel == "quantize_rows") {  // ints: activation, gated
+    const int x = in(0);
+    const auto xs = shape_of(x);
+    const int64_t columns = xs.back(), n = op.ints[1] ? columns / 2 : columns;
+    auto lead = std::vector<int64_t>(xs.begin(), xs.end() - 1), os = lead;
+    os.push_back(n);
+    bind_shape(out0, os, "quantize_rows output");
+    bind_shape(op.outputs[1], lead, "quantize_rows scale");
+    if (!launch) return;
+    int64_t rows = 1;
+    for (int64_t d : lead) rows *= d;
+    check(b200ait_quantize_rows(ptr_of(out0), static_cast<float*>(ptr_of(op.outputs[1])), ptr_of(x), rows, n, columns, n,
+                                static_cast<int>(op.ints[0]), static_cast<int>(op.ints[1]), T[x].dtype, stream),
+          op);
+    return;
+  }
+  if (op.kernel == "gemm_rcr_i8") {  // operands: x, its scales (none: x has 16 bits), w, its scales, bias, d0, d1; ints: epilogue
+    const int x = in(0), x_scale = in(1), w = in(2);
+    const auto xs = shape_of(x), ws = shape_of(w);
+    const int64_t k = xs.back(), n = ws[0];
+    if (ws[1] != k) throw Error("gemm '" + op.name + "': K mismatch");
+    std::vector<int64_t> lead(xs.begin(), xs.end() - 1), os = lead;
+    os.push_back(n);
+    int64_t m = 1;
+    for (int64_t d : lead) m *= d;
+    if (x_scale >= 0 && numel_of(x_scale) != m) throw Error("gemm '" + op.name + "': a scale per row of x is needed");
+    bind_shape(out0, os, "gemm output");
+    if (!launch) return;
+    const float* w_scale = static_cast<const float*>(ptr_of(in(3)));
+    const int epilogue = static_cast<int>(op.ints[0]);
+    const int64_t padded = (k + 15) / 16 * 16;  // (the pitch of a single row is of no account)
+    const int64_t ldb = n == 1 ? padded : k;
+    if (x_scale >= 0) {
+      check(b200ait_gemm_rcr_i8(ptr_of(x), static_cast<const float*>(ptr_of(x_scale)), ptr_of(w), w_scale, ptr_of(in(4)), ptr_of(in(5)),
+                                ptr_of(in(6)), ptr_of(out0), m, n, k, m == 1 ? padded : k, ldb, n, n, epilogue, T[out0].dtype, 0, stream),
+            op);
+      return;
+    }
+    check(b200ait_gemm_rcr_i8_x16(ptr_of(x), T[x].dtype, ptr_of(w), w_scale, ptr_of(in(4)), ptr_of(in(5)), ptr_of(in(6)), ptr_of(out0), m,
+                                  n, k, k, ldb, n, n, epilogue, T[out0].dtype, 0, workspace_, workspace_bytes_, stream),
+          op);
+    return;
+  }
+  if (op.kernel == "residual_norm") {  // ints: norm after the block, norm, 8-bit result, the sum is wanted; floats: residual's scale, eps
+    const int x = in(0);
+    const auto xs = shape_of(x);
+    const bool quantize = op.ints[2] != 0;
+    bind_shape(out0, xs, "residual_norm sum");
+    bind_shape(op.outputs[1], xs, "residual_norm output");
+    const std::vector<int64_t> lead(xs.begin(), xs.end() - 1);
+    if (quantize) bind_shape(op.outputs[2], lead, "residual_norm scale");
+    if (!launch) return;
+    const int64_t n = xs.back();
+    int64_t rows = 1;
+    for (int64_t d : lead) rows *= d;
+    auto vectors = [&](int t) { return t < 0 ? int64_t{1} : numel_of(t) / n; };
+    check(b200ait_residual_norm(op.ints[3] ? ptr_of(out0) : nullptr, ptr_of(op.outputs[1]),
+                                quantize ? static_cast<float*>(ptr_of(op.outputs[2])) : nullptr, ptr_of(x), ptr_of(in(1)), ptr_of(in(2)),
+                                ptr_of(in(3)), ptr_of(in(4)), ptr_of(in(5)), ptr_of(in(6)), rows, n, vectors(in(2)), vectors(in(5)),
+                                vectors(in(6)), n, static_cast<int>(op.ints[0]), static_cast<int>(op.ints[1]),
+                                static_cast<float>(op.floats[0]), static_cast<float>(op.floats[1]), T[x].dtype, stream),
           op);
     return;
   }

@@ -578,6 +578,7 @@ struct Side {
         case at::kInt: dtype = AITemplateDtype::kInt; break;
         case at::kLong: dtype = AITemplateDtype::kLong; break;
         case at::kBool: dtype = AITemplateDtype::kBool; break;
+        case at::kChar: dtype = AITemplateDtype::kInt8; break;
         default: return false;
       }
       names[i] = name, tensors[i] = t, given_order.push_back(static_cast<size_t>(i));

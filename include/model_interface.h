@@ -47,6 +47,7 @@ enum class AITemplateDtype {
   kLong,
   kBool,
   kBFloat16,
+  kInt8,  // not in the reference: operands of the 8-bit products
 };
 
 struct AITData {
