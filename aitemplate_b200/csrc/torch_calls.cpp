@@ -11,7 +11,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -405,16 +405,19 @@ bool on_current_device(std::initializer_list<const at::Tensor*> tensors) {
   return true;
 }
 int64_t padded(int64_t n) { return (n + 15) / 16 * 16; }
+// An uninitialised tensor on the current device, without a trip through the dispatcher (the calls below return up to three and have
+// little else to do on the host: 0.4 us each).
+at::Tensor fresh(c10::IntArrayRef shape, at::ScalarType type) {
+  return at::detail::empty_cuda(shape, type, c10::Device(c10::kCUDA, c10::cuda::current_device()), c10::nullopt);
+}
 // int8 of like's shape but rows of n, which start on 16 bytes
 at::Tensor int8_rows(const at::Tensor& like, int64_t n) {
   std::vector<int64_t> shape(like.sizes().begin(), like.sizes().end());
   shape.back() = padded(n);
-  at::Tensor q = at::empty(shape, like.options().dtype(at::kChar));
+  at::Tensor q = fresh(shape, at::kChar);
   return n == shape.back() ? q : q.narrow(-1, 0, n);
 }
-at::Tensor row_scales(const at::Tensor& like) {
-  return at::empty(like.sizes().slice(0, static_cast<size_t>(like.dim() - 1)), like.options().dtype(at::kFloat));
-}
+at::Tensor row_scales(const at::Tensor& like) { return fresh(like.sizes().slice(0, static_cast<size_t>(like.dim() - 1)), at::kFloat); }
 PyObject* tuple_of(std::initializer_list<at::Tensor> tensors) {
   PyObject* result = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
   Py_ssize_t i = 0;
@@ -483,7 +486,7 @@ PyObject* gemm_rcr_i8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
           x_scale->sizes() != x->sizes().slice(0, static_cast<size_t>(x->dim() - 1)))
         return unhandled();
       if (m == 1) lda = padded(k);
-      at::Tensor y = at::empty(shape, x->options().dtype(type));
+      at::Tensor y = fresh(shape, type);
       if (unlocked([&] {
             return lib.gemm_rcr_i8(pointer(x), static_cast<const float*>(pointer(x_scale)), pointer(w),
                                    static_cast<const float*>(pointer(w_scale)), pointer(bias), pointer(d0), pointer(d1), y.data_ptr(), m,
@@ -493,10 +496,10 @@ PyObject* gemm_rcr_i8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       return THPVariable_Wrap(std::move(y));
     }
     if (x_scale || dtype_code(*x) == 0) return unhandled();
-    at::Tensor y = at::empty(shape, x->options().dtype(type)), scratch;
+    at::Tensor y = fresh(shape, type), scratch;
     int64_t bytes = 0;
     if (lib.x16_scratch_bytes(pointer(w), m, n, k, ldb, static_cast<int>(tile_n), &bytes) != 0) return unhandled();
-    if (bytes != 0) scratch = at::empty({bytes}, x->options().dtype(at::kByte));
+    if (bytes != 0) scratch = fresh({bytes}, at::kByte);
     if (unlocked([&] {
           return lib.gemm_rcr_i8_x16(pointer(x), dtype_code(*x), pointer(w), static_cast<const float*>(pointer(w_scale)), pointer(bias),
                                      pointer(d0), pointer(d1), y.data_ptr(), m, n, k, lda, ldb, n, n, static_cast<int>(epilogue),
@@ -533,11 +536,11 @@ PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     }
     if (post == 0 && (t[2] != nullptr || t[3] != nullptr)) return unhandled();
     const bool quantize = args[11] == Py_True;
-    at::Tensor total = at::empty_like(*x), y, scale;
+    at::Tensor total = fresh(x->sizes(), x->scalar_type()), y, scale;
     if (quantize)
       y = int8_rows(*x, n), scale = row_scales(*x);
     else
-      y = at::empty_like(*x);
+      y = fresh(x->sizes(), x->scalar_type());
     const b200ait_stream_t stream = current_stream();
     if (unlocked([&] {
           return lib.residual_norm(total.data_ptr(), y.data_ptr(), quantize ? static_cast<float*>(scale.data_ptr()) : nullptr, pointer(x),
