@@ -60,8 +60,14 @@ __device__ __forceinline__ void normalize_row(const RowTeam<CNT, THREADS, ALIGNE
   by_pairs<CNT * 8>(v, [&](uint64_t x, int) { return mul2(x, pack2(rstd, rstd)); });
 }
 
+// Registers for 1024 threads an SM (64) where a block has half as many, so that two of them take turns between memory and barriers
+// (4000 x 16384 to 8 bits 101 -> 76 us), and for skewed rows (8192 x 5001 111 -> 102); else for 768 (8192 x 8192 with both norms 86 us, 88
+// with 64 registers).
+template <int THREADS, bool ALIGNED>
+constexpr int kNormBlocksPerSm = (THREADS >= 512 || !ALIGNED ? 1024 : 768) / kTeamBlock<THREADS>;
+
 template <int CNT, int THREADS, bool ALIGNED, bool QUANTIZE, bool BF16>
-__global__ void __launch_bounds__(kTeamBlock<THREADS>) residual_norm_kernel(const ResidualNormParams p) {
+__global__ void __launch_bounds__(kTeamBlock<THREADS>, (kNormBlocksPerSm<THREADS, ALIGNED>)) residual_norm_kernel(const ResidualNormParams p) {
   grid_release();
   grid_wait();
   using Team = RowTeam<CNT, THREADS, ALIGNED>;
