@@ -221,7 +221,9 @@ static void launch_residual_norm(const ResidualNormParams& p, cudaStream_t strea
 
 template <bool QUANTIZE, bool BF16>
 static void residual_norm_dispatch(const ResidualNormParams& p, bool lie_well, bool aligned, cudaStream_t stream) {
-  const TeamShape t = team_shape(p.rows, p.n, aligned, sm_count());
+  // us with one / two / four units a thread, to 8 bits: 100 x 1024 2.3 / 2.1 / 2.5, x 4096 2.6 / 2.4 / 2.4, x 8192 3.9 / 3.4 / 3.3; with both norms
+  // 100 x 2048 3.3 / 3.1 / 3.5, 333 x 4096 5.3 / 4.9 / 5.2, 600 x 4096 8.4 / 7.1 / 6.1, 2000 x 1280 10.0 / 7.6 / 7.0
+  const TeamShape t = team_shape(p.rows, p.n, aligned, 2ll * sm_count(), 2);
   if (t.cnt == 0 || !lie_well) {
     count_launch();
     residual_norm_long_rows_kernel<QUANTIZE, BF16><<<static_cast<unsigned>(p.rows), kTeamMaxThreads, 0, stream>>>(p);

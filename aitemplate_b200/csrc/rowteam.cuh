@@ -257,16 +257,16 @@ __device__ __forceinline__ int8_t quantize_value(const RowScale& s, float v) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// How a row of n elements is laid over threads: `cnt` units each; 0: the row is too long and is walked.
+// How a row of n elements is laid over threads: `cnt` units each; 0: the row is too long and is walked. Many rows are a matter of bytes in
+// flight: up to four units a thread. Up to `few_rows` of them are one of latency, and a thread takes no more than `few`.
 struct TeamShape {
   int cnt, threads;
   bool aligned;
 };
-inline TeamShape team_shape(long long rows, long long n, bool aligned, int sms) {
+inline TeamShape team_shape(long long rows, long long n, bool aligned, long long few_rows, int few) {
   const long long units = aligned ? n / 8 : (n + 14) / 8;
   if (units > (aligned ? 4 : 3) * kTeamMaxThreads) return TeamShape{0, kTeamMaxThreads, aligned};
-  // A few rows are a matter of latency: a unit a thread. Many are one of bytes in flight: up to four.
-  const long long per = rows <= 2ll * sms && units <= kTeamMaxThreads ? 1 : 4;
+  const long long per = rows <= few_rows && units <= few * kTeamMaxThreads ? few : 4;
   int threads = 32;
   while (threads * per < units) threads *= 2;
   if (!aligned && threads * 3 < units) threads *= 2;  // (skewed rows take registers)
