@@ -431,6 +431,69 @@ __device__ __forceinline__ void store_box_rows(const GemmParams& p, const uint8_
   }
 }
 
+// The same two for the 8-bit kernels (row-major outputs), with as little code and as few instructions as it takes: the code runs once
+// or a few times per launch, from a cold instruction cache, and behind short main loops a row's 45 instructions set the pace. What a
+// row needs goes by whether it starts on 4 bytes, so rows are taken one kind after the other. 777 x 1283 x 256 8.1 -> 6.7 us (777 x 1288 x
+// 256, whose rows TMA can describe, 3.6), 16384 x 777 x 512 40 -> 34 (registers matter as much: with 227 KB of shared memory in use a spilled one comes back from L2).
+template <bool BF16>
+__device__ __forceinline__ void load_box_rows_i8(uint8_t* box, const typename Elem16<BF16>::T* src, long long ld, int rows,
+                                                 int width, int lane) {
+  using T = typename Elem16<BF16>::T;
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += 8) {  // eight rows of both halves of the box, their loads before the first store
+    T x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = r0 + (i >> 1), col = (i & 1) * 32 + lane;
+      if (r < rows && col < width) x[i] = src[r * ld + col];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = r0 + (i >> 1), col = (i & 1) * 32 + lane;
+      if (r < rows && col < width) *reinterpret_cast<T*>(box + r * 128 + (((col >> 3) ^ (i >> 1)) * 16) + (col & 7) * 2) = x[i];
+    }
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void store_box_rows_i8(const GemmParams& p, const uint8_t* box, int row0, int gcol, int rows, int width,
+                                                  int lane) {
+  uint16_t* dst0 = static_cast<uint16_t*>(p.out) + static_cast<long long>(row0) * p.ldc + gcol;
+  const int off0 = static_cast<int>(reinterpret_cast<uintptr_t>(dst0) >> 1) & 1;
+  // Rows r0, r0 + step, .., which start `off` elements after a 4-byte boundary: a lane stores the pair of columns at 2 lane - off. With
+  // off = 1 lane 0 has the first column (in the upper half) and the last one.
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    const bool odd = (p.ldc & 1) != 0;
+    if (half == 1 && !odd) break;
+    const int step = odd ? 2 : 1, off = off0 ^ half;
+    const int col = 2 * lane - off;
+    const bool pair = col >= 0 && col + 1 < width, single = !pair && col >= 0 && col < width;
+    uint16_t* dst = dst0 + half * p.ldc + col;
+    const uint8_t* src = box + (lane & 3) * 4;
+#pragma unroll 1
+    for (int r0 = half; r0 < rows; r0 += 4 * step) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // (rows past the last one hold anything and go nowhere)
+        const int r = r0 + i * step;
+        w[i] = *reinterpret_cast<const uint32_t*>(src + r * 128 + (((lane >> 2) ^ (r & 7)) << 4));
+      }
+      if (off) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __shfl_sync(0xffffffffu, w[i], (lane + 31) & 31) >> 16 | w[i] << 16;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i, dst += step * p.ldc) {
+        if (r0 + i * step >= rows) break;
+        if (pair) *reinterpret_cast<uint32_t*>(dst) = w[i];
+        if (single) dst[0] = static_cast<uint16_t>(w[i]);
+        if (col < 0) dst[1] = static_cast<uint16_t>(w[i] >> 16);
+        if (col < 0 && width == 64) dst[64] = static_cast<uint16_t>(w[i]);
+      }
+    }
+  }
+}
+
 // I8: operands of signed 8-bit integers with a scale per row of A and per row of B (p.row_scale, p.col_scale), 32-bit integer sums,
 // results in 16 bits. Sums are exact, so a result does not depend on the tile or on how K is shared out.
 // BMN: B is stored [K, N]. MULTI: the staged store goes to p.num_out destinations. Both are compile-time, so that
@@ -756,7 +819,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
           for (int q = 0; q < 4; ++q) d0v[q] = reinterpret_cast<const uint4*>(d0_row + col0)[q];
         }
       };
-      if (splits == 1 && !box_d0) prefetch_d0(colh);
+      if (splits == 1 && !box_d0 && !(I8 && EPI == kRowsEpilogue)) prefetch_d0(colh);
       ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, kDevWaitAccFullTimeout);
       if (!ok) break;
       tc_fence_after();
@@ -767,6 +830,71 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
       uint32_t ra[32], rb[32];
       bool released = false;
       tmem_ld_32x32b_x32(t_base, ra);
+      auto scale_i8 = [&](float (&v)[32], int c) {
+        const float* cs = scale_s + half * (BN / 2) + c * 32;
+        const uint64_t rs = pack2(row_scale, row_scale);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const float2 f = *reinterpret_cast<const float2*>(cs + q * 2);
+          const uint64_t x = mul2(pack2(v[q * 2], v[q * 2 + 1]), pack2(f.x, f.y));
+          if (has_bias) {
+            const float2 g = *reinterpret_cast<const float2*>(bias_s + half * (BN / 2) + c * 32 + q * 2);
+            unpack2(fma2(x, rs, pack2(g.x, g.y)), v[q * 2], v[q * 2 + 1]);
+          } else {
+            unpack2(mul2(x, rs), v[q * 2], v[q * 2 + 1]);
+          }
+        }
+      };
+      if constexpr (I8 && EPI == kRowsEpilogue) {
+        uint8_t* row_base = my_staging + lane * 128;
+        const int rows = min(32, p.M - row0);
+        const bool row_d0 = has_d0 && epi_b2(code) == kBinaryNone;  // (here rows are never whole vectors)
+#pragma unroll 1
+        for (int c = 0; c < kChunksPerWarp; ++c) {
+          const int col0 = colh + c * 32, gcol = colh + (c & ~1) * 32;
+          const bool last = c + 1 == kChunksPerWarp || col0 + 32 >= p.N;  // (the first chunk of a half past the edge too)
+          if (c > 0) tmem_ld_32x32b_x32(t_base + static_cast<uint32_t>(c * 32), ra);
+          tmem_ld_wait();
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __int2float_rn(static_cast<int>(ra[j]));
+          if (last) {
+            tc_fence_before();
+            if (PAIR) {
+              mbar_arrive_cluster_relaxed(acc_empty_leader[acc]);
+            } else {
+              mbar_arrive(&acc_empty[acc]);
+            }
+          }
+          if (col0 >= p.N) break;  // warp-uniform
+          scale_i8(v, c);
+          const int width = min(64, min(BN / 2 - (c & ~1) * 32, p.N - gcol));
+          uint4 d0c[4] = {};
+          if (row_d0) {
+            if ((c & 1) == 0) {
+              load_box_rows_i8<BF16>(my_staging, static_cast<const T*>(p.d0) + static_cast<long long>(row0) * p.ldd + gcol, p.ldd, rows,
+                                     width, lane);
+              __syncwarp();
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              d0c[u] = *reinterpret_cast<const uint4*>(row_base + ((((c & 1) * 4 + u) ^ (lane & 7)) * 16));
+          }
+          epilogue_math32<BF16, EPI, I8>(p, v, d0c, b, row, col0, row_d0, row_ok);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<uint4*>(row_base + ((((c & 1) * 4 + u) ^ (lane & 7)) * 16)) = pack8<BF16>(&v[u * 8]);
+          if ((c & 1) != 0 || last) {
+            __syncwarp();
+            store_box_rows_i8<BF16>(p, my_staging, row0, gcol, rows, width, lane);
+            __syncwarp();
+          }
+          if (last) break;
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+        continue;
+      }
       auto chunk_step = [&](const int c, uint32_t (&cur)[32], uint32_t (&nxt)[32]) {
         if (!ok) return;
         const int col0 = colh + c * 32;
@@ -810,19 +938,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
           return;
         }
         if constexpr (I8) {
-          const float* cs = scale_s + half * (BN / 2) + c * 32;
-          const uint64_t rs = pack2(row_scale, row_scale);
-#pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const float2 f = *reinterpret_cast<const float2*>(cs + q * 2);
-            const uint64_t x = mul2(pack2(v[q * 2], v[q * 2 + 1]), pack2(f.x, f.y));
-            if (has_bias) {
-              const float2 g = *reinterpret_cast<const float2*>(bias_s + half * (BN / 2) + c * 32 + q * 2);
-              unpack2(fma2(x, rs, pack2(g.x, g.y)), v[q * 2], v[q * 2 + 1]);
-            } else {
-              unpack2(mul2(x, rs), v[q * 2], v[q * 2 + 1]);
-            }
-          }
+          scale_i8(v, c);
         } else if (!kLean && p.alpha != 1.f) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= p.alpha;
