@@ -908,18 +908,19 @@ B200AIT_EXPORT int b200ait_gemm_rcr(const void* a, const void* b, const void* bi
   });
 }
 
-static void check_i8(int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb, int64_t ldc, int64_t ldd, int epilogue) {
+static void check_i8(const GemmArgs& g, const float* b_scale) {
+  B200AIT_REQUIRE(g.dtype == kDTypeHalf || g.dtype == kDTypeBFloat16, "gemm: dtype must be float16 or bfloat16");
+  B200AIT_REQUIRE(g.m >= 0 && g.n >= 0 && g.k >= 0, "gemm: negative dimension");
   // sums of K products of at most 2^14 each stay below 2^31
-  B200AIT_REQUIRE(k < (1 << 17), "gemm: 8-bit operands take up to 131071 columns");
-  if (m <= 0 || n <= 0) return;
-  B200AIT_REQUIRE(k != 0, "gemm: 8-bit operands have no columns");
-  B200AIT_REQUIRE(k < 0 || (lda >= k && ldb >= k && ldc >= n), "gemm: a row pitch is shorter than the row");
-  const bool residual = epi_b1(epilogue) != kBinaryNone || epi_b2(epilogue) != kBinaryNone;
-  B200AIT_REQUIRE(!residual || ldd >= n, "gemm: a row pitch is shorter than the row");
-}
-static void check_scale(const float* scale) {
-  B200AIT_REQUIRE(scale != nullptr, "gemm: 8-bit operands need the scales of their rows");
-  B200AIT_REQUIRE((reinterpret_cast<uintptr_t>(scale) & 3u) == 0, "gemm: a pointer is not aligned to its type");
+  B200AIT_REQUIRE(g.k < (1 << 17), "gemm: 8-bit operands take up to 131071 columns");
+  if (g.m == 0 || g.n == 0) return;
+  B200AIT_REQUIRE(g.k != 0, "gemm: 8-bit operands have no columns");
+  B200AIT_REQUIRE(g.a && g.b && g.c, "gemm: null operand pointer with non-zero size");
+  B200AIT_REQUIRE(b_scale != nullptr, "gemm: 8-bit operands need the scales of their rows");
+  const bool residual = epi_b1(g.epilogue) != kBinaryNone || epi_b2(g.epilogue) != kBinaryNone;
+  B200AIT_REQUIRE(g.lda >= g.k && g.ldb >= g.k && g.ldc >= g.n && (!residual || g.ldd >= g.n), "gemm: a row pitch is shorter than the row");
+  auto at = [](const void* ptr, unsigned bytes) { return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0; };
+  B200AIT_REQUIRE(at(g.bias, 2) && at(g.d0, 2) && at(g.d1, 2) && at(g.c, 2) && at(b_scale, 4), "gemm: a pointer is not aligned to its type");
 }
 
 // gemm_rcr of signed 8-bit integers: c = epilogue(sum_k a[m, k] b[n, k] * a_scale[m] * b_scale[n] + bias, d0, d1).
@@ -928,9 +929,10 @@ B200AIT_EXPORT int b200ait_gemm_rcr_i8(const void* a, const float* a_scale, cons
                                        int64_t k, int64_t lda, int64_t ldb, int64_t ldc, int64_t ldd, int epilogue, int dtype,
                                        int tile_n, cudaStream_t stream) {
   return guarded("b200ait_gemm_rcr_i8", [&] {
-    check_i8(m, n, k, lda, ldb, ldc, ldd, epilogue);
     GemmArgs g{a, b, bias, d0, d1, c, 1, m, n, k, lda, ldb, ldc, ldd, 0, 0, 0, 0, epilogue, dtype, 1.f, 0, 1, 1, 1, tile_n, stream};
-    if (m > 0 && n > 0) check_scale(a_scale), check_scale(b_scale);
+    check_i8(g, b_scale);
+    B200AIT_REQUIRE(m == 0 || n == 0 || a_scale, "gemm: 8-bit operands need the scales of their rows");
+    B200AIT_REQUIRE((reinterpret_cast<uintptr_t>(a_scale) & 3u) == 0, "gemm: a pointer is not aligned to its type");
     g.i8 = 1, g.row_scale = a_scale, g.col_scale = b_scale;
     gemm_run(g);
   });
@@ -956,12 +958,10 @@ B200AIT_EXPORT int b200ait_gemm_rcr_i8_x16(const void* x, int x_dtype, const voi
                                            int64_t scratch_bytes, cudaStream_t stream) {
   return guarded("b200ait_gemm_rcr_i8_x16", [&] {
     B200AIT_REQUIRE(x_dtype == kDTypeHalf || x_dtype == kDTypeBFloat16, "gemm: x must be float16 or bfloat16");
-    check_i8(m, n, k, ldx, ldb, ldc, ldd, epilogue);
-    if (m <= 0 || n <= 0) B200AIT_REQUIRE(m >= 0 && n >= 0, "gemm: negative dimension");
-    if (m == 0 || n == 0) return;
-    check_scale(b_scale);
-    B200AIT_REQUIRE(x && (reinterpret_cast<uintptr_t>(x) & 1u) == 0, "gemm: x is null or not aligned to its type");
     GemmArgs g{x, b, bias, d0, d1, c, 1, m, n, k, ldx, ldb, ldc, ldd, 0, 0, 0, 0, epilogue, dtype, 1.f, 0, 1, 1, 1, tile_n, stream};
+    check_i8(g, b_scale);
+    if (m == 0 || n == 0) return;
+    B200AIT_REQUIRE((reinterpret_cast<uintptr_t>(x) & 1u) == 0, "gemm: a pointer is not aligned to its type");
     g.i8 = 1, g.col_scale = b_scale;
     const int64_t needed = x16_scratch_bytes(m, n, k, ldb, b, tile_n);
     if (needed == 0) {

@@ -25,7 +25,9 @@ def _gemm(a=P, a_scale=P, b=P, b_scale=P, bias=None, d0=None, d1=None, c=P, m=4,
     (dict(k=131072, lda=131072, ldb=131072), "131071"), (dict(lda=31), "pitch"), (dict(ldb=16), "pitch"), (dict(ldc=7), "pitch"),
     (dict(epilogue=1 << 4, d0=P, ldd=4), "pitch"), (dict(epilogue=1 << 4), "needs d0"), (dict(epilogue=1 << 6, d0=P), "needs d1"),
     (dict(a_scale=None), "scales"), (dict(b_scale=None), "scales"), (dict(a=None), "null operand"), (dict(c=None), "null operand"),
-    (dict(dtype=F32), "dtype"), (dict(m=-1), "negative"), (dict(k=0), "no columns"),
+    (dict(dtype=F32), "dtype"), (dict(m=-1), "negative"), (dict(k=0), "no columns"), (dict(c=ctypes.c_void_p(4097)), "aligned to its type"),
+    (dict(bias=ctypes.c_void_p(4097)), "aligned to its type"), (dict(b_scale=ctypes.c_void_p(4098)), "aligned to its type"),
+    (dict(a_scale=ctypes.c_void_p(4098)), "aligned to its type"),
 ])
 def test_gemm_rcr_i8_refuses(change, said):
     _refused("b200ait_gemm_rcr_i8", _gemm(**change), said)
@@ -36,6 +38,29 @@ def test_gemm_rcr_i8_of_nothing():
     assert _lib.load().b200ait_gemm_rcr_i8(*_gemm(b=None, b_scale=None, c=None, n=0)) == 0
 
 
+def _x16(x=P, x_dtype=F16, b=P, b_scale=P, bias=None, d0=None, d1=None, c=P, m=8, n=8, k=32, ldx=32, ldb=32, ldc=8, ldd=8, epilogue=0,
+         dtype=F16, tile_n=0, scratch=P, scratch_bytes=8 * 36):
+    return [x, x_dtype, b, b_scale, bias, d0, d1, c, m, n, k, ldx, ldb, ldc, ldd, epilogue, dtype, tile_n, scratch, scratch_bytes, None]
+
+
+@pytest.mark.parametrize("change,said", [
+    (dict(x_dtype=F32), "x must be"), (dict(dtype=F32), "dtype"), (dict(scratch=None), "scratch"), (dict(scratch_bytes=8 * 36 - 1), "scratch"),
+    (dict(scratch=ctypes.c_void_p(4104)), "scratch"), (dict(x=ctypes.c_void_p(4097)), "aligned to its type"), (dict(x=None), "null operand"),
+    (dict(b_scale=None), "scales"), (dict(ldx=31), "pitch"), (dict(k=131072, ldx=131072, ldb=131072), "131071"), (dict(n=-1), "negative"),
+])
+def test_gemm_rcr_i8_x16_refuses(change, said):
+    _refused("b200ait_gemm_rcr_i8_x16", _x16(**change), said)
+
+
+def test_scratch_of_16_bit_rows():
+    lib, out = _lib.load(), ctypes.c_int64(-1)
+    for (m, n, k, ldb, b, tile), want in {(8, 8, 33, 48, 4096, 0): 8 * 48 + 32, (1, 8, 33, 48, 4096, 0): 0, (1, 8, 33, 40, 4096, 0): 52,
+                                          (1, 8, 33, 48, 4104, 0): 52, (1, 8, 33, 48, 4096, 64): 52, (0, 8, 33, 48, 4096, 0): 0,
+                                          (4, 4096, 4096, 4096, 4096, 0): 4 * 4100, (4, 1024, 1024, 1024, 4096, 0): 0}.items():
+        assert lib.b200ait_gemm_rcr_i8_x16_scratch_bytes(b, m, n, k, ldb, tile, ctypes.byref(out)) == 0
+        assert out.value == want, (m, n, k)
+
+
 def _quantize(q=P, scale=P, x=P, rows=2, n=16, x_pitch=16, q_pitch=16, activation=0, gated=0, dtype=F16):
     return [q, scale, x, rows, n, x_pitch, q_pitch, activation, gated, dtype, None]
 
@@ -43,7 +68,8 @@ def _quantize(q=P, scale=P, x=P, rows=2, n=16, x_pitch=16, q_pitch=16, activatio
 @pytest.mark.parametrize("change,said", [
     (dict(dtype=F32), "dtype"), (dict(rows=-1), "negative"), (dict(activation=8), "activation"), (dict(activation=-1), "activation"),
     (dict(x=None), "null"), (dict(scale=None), "null"), (dict(x_pitch=15), "pitch"), (dict(q_pitch=15), "pitch"),
-    (dict(gated=1), "pitch"), (dict(rows=1 << 31), "int32"),
+    (dict(gated=1), "pitch"), (dict(rows=1 << 31), "int32"), (dict(x=ctypes.c_void_p(4097)), "aligned to its type"),
+    (dict(scale=ctypes.c_void_p(4098)), "aligned to its type"),
 ])
 def test_quantize_rows_refuses(change, said):
     _refused("b200ait_quantize_rows", _quantize(**change), said)
@@ -59,6 +85,8 @@ def _norm(sum=P, y=P, y_scale=None, x=P, residual=None, gate=None, post_gamma=No
     (dict(dtype=F32), "dtype"), (dict(norm=0), "layer (1) or rms (2)"), (dict(norm=3), "layer (1) or rms (2)"), (dict(post_norm=3), "none (0)"),
     (dict(post_gamma=P), "need a norm"), (dict(x=None), "null"), (dict(y=None), "null"), (dict(gate=P, gates=4), "each gate"),
     (dict(gamma=P, gammas=0), "each gamma"), (dict(beta=P, betas=5), "each beta"), (dict(y_scale=P, y_pitch=8), "pitch"), (dict(n=-1), "negative"),
+    (dict(gamma=ctypes.c_void_p(4097)), "aligned to its type"), (dict(y=ctypes.c_void_p(4097)), "aligned to its type"),
+    (dict(y_scale=ctypes.c_void_p(4098)), "aligned to its type"),
 ])
 def test_residual_norm_refuses(change, said):
     _refused("b200ait_residual_norm", _norm(**change), said)

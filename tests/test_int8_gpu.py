@@ -626,6 +626,29 @@ def test_the_native_path_and_the_python_code_agree(monkeypatch):
             assert p.shape == q.shape and p.dtype == q.dtype and p.stride() == q.stride() and torch.equal(p, q)
 
 
+def test_another_device_is_refused(monkeypatch):
+    x, w, ws, xs, *_ = _problem(6, 32, 64, torch.float16, "", False, 1)
+
+    class Absent:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    monkeypatch.setattr(kernels, "_calls", Absent())
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    for call in (lambda: kernels.gemm_rcr_i8(x, w, ws, xs), lambda: kernels.quantize_rows(xs), lambda: kernels.residual_norm(xs)):
+        with pytest.raises(ValueError, match="the current device is cuda:1"):
+            call()
+
+
+def test_one_dimension():
+    x, w, ws, xs, b, _, _ = _problem(1, 40, 64, torch.float16, "", True, 1)
+    assert torch.equal(kernels.gemm_rcr_i8(x[0], w, ws, xs[0], bias=b), kernels.gemm_rcr_i8(x, w, ws, xs, bias=b)[0])
+    v = torch.randn(70, generator=_gen(1), device="cuda").half()
+    (q, s), (q2, s2) = kernels.quantize_rows(v), kernels.quantize_rows(v[None])
+    assert q.shape == (70,) and s.shape == () and torch.equal(q, q2[0]) and torch.equal(s, s2[0])
+    assert torch.equal(kernels.residual_norm(v)[1], kernels.residual_norm(v[None])[1][0])
+
+
 def test_refusals():
     x, w, ws, xs, b, d0, _ = _problem(6, 32, 64, torch.float16, "add", True, 1)
     call = kernels.gemm_rcr_i8
