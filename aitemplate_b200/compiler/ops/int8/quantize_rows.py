@@ -3,8 +3,8 @@
     q, scale = quantize_rows(activation="identity", gated=False)(x)
 
 scale = max |v| / 127 and q = round(127 v / max |v|), ties to even, with v = act(x), or with `gated` v = act(x[..., :n]) * x[..., n:]
-for the two halves of a gated feed-forward's first product. q and scale are operands of gemm_rcr_i8. A row of zeros has scale 0, a
-row with an infinity or a NaN in it scale NaN (and q 0). The reference has no 8-bit activations; the activations are those of
+for the two halves of a gated feed-forward's first product. q and scale are operands of gemm_rcr_i8. A row of v that is all zeros has
+scale 0, one with an infinity or a NaN in it scale NaN (and q 0). The reference has no 8-bit activations; the activations are those of
 its GEMM epilogues."""
 from __future__ import annotations
 

@@ -116,12 +116,15 @@ __device__ __forceinline__ void apply_unary_vec(int u, float (&v)[N]) {
 // with it.
 __device__ __forceinline__ uint64_t gelu2(uint64_t x) {
   auto both = [](float c) { return pack2(c, c); };
-  float x0, x1, e0, e1, d0, d1;
+  float x0, x1, m0, m1, e0, e1, d0, d1;
   unpack2(x, x0, x1);
-  unpack2(mul2(mul2(x, x), both(-0.72134752f)), e0, e1);  // exp(-x^2 / 2) = 2^(-x^2 log2(e) / 2)
+  // |x| up to 16, where erfc is 0 in 32 bits (an infinity must not meet that 0); a NaN stays one
+  asm("min.NaN.f32 %0, %1, 0f41800000;" : "=f"(m0) : "f"(fabsf(x0)));
+  asm("min.NaN.f32 %0, %1, 0f41800000;" : "=f"(m1) : "f"(fabsf(x1)));
+  const uint64_t m = pack2(m0, m1);
+  unpack2(mul2(mul2(m, m), both(-0.72134752f)), e0, e1);  // exp(-x^2 / 2) = 2^(-x^2 log2(e) / 2)
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e1));
-  const uint64_t m = pack2(fabsf(x0), fabsf(x1));
   unpack2(fma2(m, both(0.3275911f * 0.70710678f), both(1.f)), d0, d1);
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d0));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d1));

@@ -129,7 +129,8 @@ int b200ait_gemm_rcr_static_scratch(const void* a, const void* b, const void* bi
  * a [m, k] (row pitch lda), b [n, k] (row pitch ldb), both int8; the scales are fp32 device vectors; bias, d0, d1 and c have the 16-bit
  * type `dtype`. Sums are exact 32-bit integers (k <= 131071), scaled and run through the epilogue in fp32, rounded once. Operands
  * that start on 16 bytes with pitches of whole 16 bytes go to the tensor cores whatever k is; others take a slower kernel.
- * tile_n as for b200ait_gemm_rcr. A scale that is NaN (b200ait_quantize_rows) makes its row NaN. No counterpart in the reference,
+ * tile_n as for b200ait_gemm_rcr. A scale that is NaN (b200ait_quantize_rows) makes its row NaN ahead of the activation (relu,
+ * here as in the other GEMMs, makes that 0). No counterpart in the reference,
  * whose GEMMs take 16- and 32-bit floats only. */
 int b200ait_gemm_rcr_i8(const void* a, const float* a_scale, const void* b, const float* b_scale, const void* bias,
                         const void* d0, const void* d1, void* c, int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb,
@@ -235,8 +236,8 @@ int b200ait_layernorm(void* out, const void* in, const void* gamma, const void* 
                       b200ait_stream_t stream);
 
 /* Rows of 16-bit values to signed 8-bit ones with a scale each: q = round(127 v / max |v|) to the nearest, ties to even, and scale =
- * max |v| / 127, with v = act(x[:, :n]), or with `gated` act(x[:, :n]) * x[:, n:2n]. A row of zeros has scale 0 and q 0, a row with
- * an infinity or a NaN scale NaN and q 0. Row pitches in elements; bytes of q between n and its pitch are left alone. `activation`:
+ * max |v| / 127, with v = act(x[:, :n]), or with `gated` act(x[:, :n]) * x[:, n:2n]. A row of v that is all zeros has scale 0 and q 0, one
+ * with an infinity or a NaN in it scale NaN and q 0 (the relu of a NaN is 0, as in the GEMMs). Row pitches in elements; bytes of q between n and its pitch are left alone. `activation`:
  * one of B200AIT_UNARY_*. No counterpart in the reference. */
 int b200ait_quantize_rows(void* q, float* scale, const void* x, int64_t rows, int64_t n, int64_t x_pitch, int64_t q_pitch,
                           int activation, int gated, int dtype, b200ait_stream_t stream);

@@ -154,6 +154,24 @@ def test_product_of_the_largest_sums():
         _close(kernels.gemm_rcr_i8(x, w, ws, xs), want, off, torch.float16)
 
 
+@pytest.mark.parametrize("epilogue", ["", "gelu", "swish", "hardswish"])
+def test_product_of_scales_that_are_no_numbers(epilogue):
+    """An infinite scale gives infinities, one that is NaN gives NaN, in its row alone and on every kernel."""
+    for m, n, k, pad, tile in ((2, 40, 64, 64, 0), (1, 130, 512, 512, 0), (9, 256, 512, 512, 0), (70, 64, 128, 128, 64), (300, 264, 128, 128, 512),
+                               (70, 131, 128, 128, 0), (20, 40, 33, 33, 0)):
+        x, w, ws, xs, b, _, _ = _problem(m, n, k, torch.float16, "", True, m, pad, pad)
+        x.abs_().clamp_(1, 127), w.abs_().clamp_(1, 127)  # (sums above 0)
+        clean = kernels.gemm_rcr_i8(x, w, ws, xs, bias=b, epilogue=epilogue, tile_n=tile)
+        for bad in (math.inf, math.nan):
+            xs2 = xs.clone()
+            xs2[m // 2] = bad
+            y = kernels.gemm_rcr_i8(x, w, ws, xs2, bias=b, epilogue=epilogue, tile_n=tile)
+            row = y[m // 2].float()
+            assert bool((row == math.inf).all() if bad == math.inf else torch.isnan(row).all()), (m, n, k, bad)
+            rest = torch.arange(m, device="cuda") != m // 2
+            assert torch.equal(y[rest], clean[rest])
+
+
 def test_product_leading_dims_and_empty():
     x, w, ws, xs, b, _, _ = _problem(24, 96, 64, torch.float16, "", True, 3)
     y = kernels.gemm_rcr_i8(x, w, ws, xs, bias=b)
