@@ -1,4 +1,4 @@
-// gemm_rcr_i8 for one to four rows of X: the run time is the time to read W once, and there is nothing for the tensor core to
+// gemm_rcr_i8 for one or two rows of X in 8 bits, one to four in 16: the run time is the time to read W once, and there is nothing for the tensor core to
 // amortise. One block per SM holds X in shared memory and owns a contiguous share of the rows of W; a warp streams R rows at a time,
 // KV 16-byte vectors of each per lane, eight vectors in flight while the eight before them are multiplied (four products per
 // instruction, exact 32-bit sums), adds up across the lanes and runs the fused epilogue. X may come in 16 bits: then every

@@ -16,7 +16,8 @@ namespace b200ait {
 enum RowNorm : int { kNormNone = 0, kNormLayer = 1, kNormRms = 2 };
 
 // Which of the vectors that rows share goes with a row: row / (rows that share one), by multiply-high with constants of the host (a
-// 64-bit division takes as long as four values: 8192 x 1280 with three of them 17.9 us, 15.6 so).
+// 64-bit division takes as long as four values: 8192 x 1280 with three of them 17.9 us, 15.6 so, both with the results of the run
+// before overwritten in L2).
 struct RowParts {
   int rows = 1;
   unsigned mul = 0, shr = 0;
