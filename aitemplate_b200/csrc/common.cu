@@ -1,6 +1,7 @@
 // Library-wide host state: last-error text, per-device status word, device properties.
 #include "common.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cstring>
 #include <mutex>
@@ -55,6 +56,22 @@ void opt_in_smem_once(std::atomic<uint64_t>& done, const void* kernel, int bytes
   const uint64_t bit = 1ull << dev;
   if (done.load(std::memory_order_acquire) & bit) return;
   B200AIT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_release);
+}
+
+void prefer_l1_once(std::atomic<uint64_t>& done, const void* kernel, int threads) {
+  const int dev = current_device();
+  const uint64_t bit = 1ull << dev;
+  if (done.load(std::memory_order_acquire) & bit) return;
+  cudaFuncAttributes about = {};
+  int blocks = 0, reserved = 0, all = 0;
+  B200AIT_CUDA_CHECK(cudaFuncGetAttributes(&about, kernel));
+  B200AIT_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, 0));
+  B200AIT_CUDA_CHECK(cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, dev));
+  B200AIT_CUDA_CHECK(cudaDeviceGetAttribute(&all, cudaDevAttrMaxSharedMemoryPerMultiprocessor, dev));
+  const int bytes = blocks * (static_cast<int>(about.sharedSizeBytes) + reserved);
+  const int percent = std::min(100, (bytes * 100 + all - 1) / all);
+  B200AIT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, percent));
   done.fetch_or(bit, std::memory_order_release);
 }
 

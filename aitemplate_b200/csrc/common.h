@@ -31,6 +31,12 @@ int sm_count();
 // Raises a kernel's dynamic shared-memory limit once per device (bit i of `done` = device i).
 void opt_in_smem_once(std::atomic<uint64_t>& done, const void* kernel, int bytes);
 
+// Has the driver set as little of an SM's memory aside as shared memory as the blocks of a kernel that fit one need, once per device; the rest is
+// L1. A kernel that streams rows has that many loads in flight as L1 takes, and one that starts early (launch_early) would otherwise
+// move in beside the CTAs of a GEMM, which leave L1 next to nothing, and keep their split to its end: residual_norm of 8192 x 4096 to 8 bits in turn with a product to 1024
+// columns 85.7 us, 73.4 so (started late 72.6), of 24576 x 768 in turn with a GEMM 59.7 and 56.7 (57.4), alone the same.
+void prefer_l1_once(std::atomic<uint64_t>& done, const void* kernel, int threads);
+
 struct Error : public std::runtime_error {
   using std::runtime_error::runtime_error;
 };

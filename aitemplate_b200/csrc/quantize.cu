@@ -89,8 +89,11 @@ template <int CNT, int THREADS, bool ALIGNED, bool GATED, bool BF16>
 static void launch_quantize(const QuantizeParams& p, cudaStream_t stream) {
   constexpr int kBlock = kTeamBlock<THREADS>;
   const long long blocks = THREADS > 32 ? p.rows : (p.rows + kTeamWarpsPerBlock - 1) / kTeamWarpsPerBlock;
+  const auto kernel = &quantize_rows_kernel<CNT, THREADS, ALIGNED, GATED, BF16>;
+  static std::atomic<uint64_t> done{0};
+  prefer_l1_once(done, reinterpret_cast<const void*>(kernel), kBlock);
   const bool early = blocks_start_early(blocks, kBlock, sm_count(), 2048) || !in_capture(stream);
-  launch_early(&quantize_rows_kernel<CNT, THREADS, ALIGNED, GATED, BF16>, dim3(static_cast<unsigned>(blocks)), kBlock, 0, stream, early, 1, p);
+  launch_early(kernel, dim3(static_cast<unsigned>(blocks)), kBlock, 0, stream, early, 1, p);
 }
 
 template <bool GATED, bool BF16>
