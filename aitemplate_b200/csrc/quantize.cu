@@ -107,7 +107,7 @@ static void quantize_dispatch(const QuantizeParams& p, bool lie_well, bool align
     B200AIT_CUDA_CHECK(cudaGetLastError());
     return;
   }
-  for_team_shape(t, [&](auto cnt, auto threads, auto whole) {
+  for_team_shape<1>(t, [&](auto cnt, auto threads, auto whole) {
     launch_quantize<decltype(cnt)::value, decltype(threads)::value, decltype(whole)::value, GATED, BF16>(p, stream);
   });
 }

@@ -63,9 +63,9 @@ __device__ __forceinline__ void normalize_row(const RowTeam<CNT, THREADS, ALIGNE
 
 // Registers for 1024 threads an SM (64) where a block has half as many, so that two of them take turns between memory and barriers
 // (4000 x 16384 to 8 bits 101 -> 76 us), and for skewed rows (8192 x 5001 111 -> 102); else for 768 (8192 x 8192 with both norms 86 us, 88
-// with 64 registers).
-template <int THREADS, bool ALIGNED>
-constexpr int kNormBlocksPerSm = (THREADS >= 512 || !ALIGNED ? 1024 : 768) / kTeamBlock<THREADS>;
+// with 64 registers). Five and six units a thread take the registers of 512 threads (8192 x 1280 with both norms 20.0, 21.0 with those of 640).
+template <int CNT, int THREADS, bool ALIGNED>
+constexpr int kNormBlocksPerSm = (CNT > 4 ? 512 : THREADS >= 512 || !ALIGNED ? 1024 : 768) / kTeamBlock<THREADS>;
 // Vectors that rows share are loaded ahead of the statistics that come before their use where that fits these registers: 8192 x 1280 with
 // both norms and a gate 21.3 -> 20.2 us, 8192 x 1536 23.5 -> 22.0; with four units a thread it would take those of 640 threads, and
 // 8192 x 4096 to 8 bits 45 -> 58, and where a warp has a row, without barriers to wait at, it gains nothing (24576 x 768 25.2, 26.2).
@@ -73,7 +73,7 @@ template <int CNT, int THREADS, bool ALIGNED>
 constexpr bool kNormLoadsAhead = ALIGNED && THREADS > 32 && THREADS <= 256 && CNT <= 3;
 
 template <int CNT, int THREADS, bool ALIGNED, bool QUANTIZE, bool BF16>
-__global__ void __launch_bounds__(kTeamBlock<THREADS>, (kNormBlocksPerSm<THREADS, ALIGNED>)) residual_norm_kernel(const ResidualNormParams p) {
+__global__ void __launch_bounds__(kTeamBlock<THREADS>, (kNormBlocksPerSm<CNT, THREADS, ALIGNED>)) residual_norm_kernel(const ResidualNormParams p) {
   grid_release();
   grid_wait();
   using Team = RowTeam<CNT, THREADS, ALIGNED>;
@@ -258,7 +258,7 @@ static void residual_norm_dispatch(const ResidualNormParams& p, bool lie_well, b
     B200AIT_CUDA_CHECK(cudaGetLastError());
     return;
   }
-  for_team_shape(t, [&](auto cnt, auto threads, auto whole) {
+  for_team_shape<2>(t, [&](auto cnt, auto threads, auto whole) {
     launch_residual_norm<decltype(cnt)::value, decltype(threads)::value, decltype(whole)::value, QUANTIZE, BF16>(p, stream);
   });
 }

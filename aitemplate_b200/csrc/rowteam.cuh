@@ -26,7 +26,7 @@
 namespace b200ait {
 
 constexpr int kTeamMaxThreads = 1024;
-constexpr int kTeamWarpsPerBlock = 8;  // rows of a block where a warp takes a row
+constexpr int kTeamWarpsPerBlock = 4;  // rows of a block where a warp takes a row
 
 template <int THREADS>
 constexpr int kTeamBlock = THREADS == 32 ? 32 * kTeamWarpsPerBlock : THREADS;
@@ -259,20 +259,34 @@ __device__ __forceinline__ int8_t quantize_value(const RowScale& s, float v) {
 
 // ------------------------------------------------------------------------------------------------ host
 // How a row of n elements is laid over threads: `cnt` units each; 0: the row is too long and is walked. Many rows are a matter of bytes in
-// flight: up to four units a thread. Up to `few_rows` of them are one of latency, and a thread takes no more than `few`.
+// flight and of lanes without a unit: up to four units a thread, five where that halves the threads, and six up to 128 of them. us, four at most and
+// so: residual_norm of 16384 x 1280 with both norms 37.6, 33.2, plain 34.4, 28.8, of 4096 x 5120 42.3, 37.1 and 38.4, 29.6, of 13648 x 1536
+// (six) 34.5, 32.7 and 31.7, 28.4; quantize_rows of 16384 x 1280 18.4, 11.3, gated 20.4, 17.0, of 1024 x 20480 21.5, 15.6; but six of 256 threads,
+// 1704 x 12288 to 8 bits 31.4, 32.8. Skewed rows take registers: up to three. Up to `few_rows` rows are a matter of latency, and a thread
+// takes no more than `few` units.
 struct TeamShape {
   int cnt, threads;
   bool aligned;
 };
-inline TeamShape team_shape(long long rows, long long n, bool aligned, long long few_rows, int few) {
-  const long long units = aligned ? n / 8 : (n + 14) / 8;
+constexpr TeamShape team_shape_of(long long units, bool aligned, bool few_rows, int few) {
   if (units > (aligned ? 4 : 3) * kTeamMaxThreads) return TeamShape{0, kTeamMaxThreads, aligned};
-  const long long per = rows <= few_rows && units <= few * kTeamMaxThreads ? few : 4;
+  const bool spread = few_rows && units <= few * kTeamMaxThreads;
   int threads = 32;
-  while (threads * per < units) threads *= 2;
-  if (!aligned && threads * 3 < units) threads *= 2;  // (skewed rows take registers)
-  const int cnt = static_cast<int>((units + threads - 1) / threads);
-  return TeamShape{cnt, threads, aligned};
+  while (threads * (spread ? few : !aligned || threads > 512 ? 4 : threads > 128 ? 5 : 6) < units) threads *= 2;
+  if (!aligned && threads * 3 < units) threads *= 2;
+  return TeamShape{static_cast<int>((units + threads - 1) / threads), threads, aligned};
+}
+inline TeamShape team_shape(long long rows, long long n, bool aligned, long long few_rows, int few) {
+  return team_shape_of(aligned ? n / 8 : (n + 14) / 8, aligned, rows <= few_rows, few);
+}
+// Does a row of any length come to this shape? (The steps between shapes lie at whole 32 units.)
+constexpr bool team_shape_is_taken(int cnt, int threads, bool aligned, int few) {
+  for (int units = 32; units <= 4 * kTeamMaxThreads; units += 32)
+    for (int i = 0; i < 2; ++i) {
+      const TeamShape t = team_shape_of(units, aligned, i != 0, few);
+      if (t.cnt == cnt && t.threads == threads) return true;
+    }
+  return false;
 }
 // Do these operands of rows at a pitch of whole elements lie alike: at the same place of 16 bytes in every row?
 inline bool lie_alike(std::initializer_list<const void*> operands) {
@@ -287,14 +301,17 @@ inline bool lie_alike(std::initializer_list<const void*> operands) {
 inline bool multiple_of(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // Calls `launch` with (CNT, THREADS, ALIGNED) as compile-time numbers.
-template <class F>
+template <int FEW, class F>
 inline void for_team_shape(const TeamShape& t, F&& launch) {
   switch (t.cnt * 10000 + t.threads + (t.aligned ? 0 : 1)) {
-#define B200AIT_TEAM(CNT, THREADS, ALIGNED)            \
-  case (CNT) * 10000 + (THREADS) + ((ALIGNED) ? 0 : 1): \
-    return launch(std::integral_constant<int, CNT>{}, std::integral_constant<int, THREADS>{}, std::integral_constant<bool, ALIGNED>{});
-#define B200AIT_TEAMS(THREADS)                                                                                   \
-  B200AIT_TEAM(1, THREADS, true) B200AIT_TEAM(2, THREADS, true) B200AIT_TEAM(3, THREADS, true) B200AIT_TEAM(4, THREADS, true) \
+#define B200AIT_TEAM(CNT, THREADS, ALIGNED)                                                                                                    \
+  case (CNT) * 10000 + (THREADS) + ((ALIGNED) ? 0 : 1):                                                                                        \
+    if constexpr (team_shape_is_taken(CNT, THREADS, ALIGNED, FEW))                                                                             \
+      return launch(std::integral_constant<int, CNT>{}, std::integral_constant<int, THREADS>{}, std::integral_constant<bool, ALIGNED>{});      \
+    break;
+#define B200AIT_TEAMS(THREADS)                                                                                                                 \
+  B200AIT_TEAM(1, THREADS, true) B200AIT_TEAM(2, THREADS, true) B200AIT_TEAM(3, THREADS, true) B200AIT_TEAM(4, THREADS, true)                  \
+  B200AIT_TEAM(5, THREADS, true) B200AIT_TEAM(6, THREADS, true)                                                                                \
   B200AIT_TEAM(1, THREADS, false) B200AIT_TEAM(2, THREADS, false) B200AIT_TEAM(3, THREADS, false)
     B200AIT_TEAMS(32) B200AIT_TEAMS(64) B200AIT_TEAMS(128) B200AIT_TEAMS(256) B200AIT_TEAMS(512) B200AIT_TEAMS(1024)
 #undef B200AIT_TEAMS
