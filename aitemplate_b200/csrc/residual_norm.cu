@@ -66,11 +66,12 @@ __device__ __forceinline__ void normalize_row(const RowTeam<CNT, THREADS, ALIGNE
 // with 64 registers). Five and six units a thread take the registers of 512 threads (8192 x 1280 with both norms 20.0, 21.0 with those of 640).
 template <int CNT, int THREADS, bool ALIGNED>
 constexpr int kNormBlocksPerSm = (CNT > 4 ? 512 : THREADS >= 512 || !ALIGNED ? 1024 : 768) / kTeamBlock<THREADS>;
-// Vectors that rows share are loaded ahead of the statistics that come before their use where that fits these registers: 8192 x 1280 with
-// both norms and a gate 21.3 -> 20.2 us, 8192 x 1536 23.5 -> 22.0; with four units a thread it would take those of 640 threads, and
-// 8192 x 4096 to 8 bits 45 -> 58, and where a warp has a row, without barriers to wait at, it gains nothing (24576 x 768 25.2, 26.2).
+// Vectors that rows share are loaded ahead of the statistics that come before their use where that fits these registers, which is where rows
+// are few: in a graph 250 x 4096 to 8 bits with both norms and a gate 4.3 -> 4.0 us, 290 x 2048 3.6 -> 3.1, 100 x 1024 2.9 -> 2.6. With four units a
+// thread it would take those of 640 threads (8192 x 4096 to 8 bits 45 -> 58), with five it gains nothing (8192 x 1280 20.0, 21.4), nor where a
+// warp has a row, without barriers to wait at (24576 x 768 25.2, 26.2).
 template <int CNT, int THREADS, bool ALIGNED>
-constexpr bool kNormLoadsAhead = ALIGNED && THREADS > 32 && THREADS <= 256 && CNT <= 3;
+constexpr bool kNormLoadsAhead = ALIGNED && THREADS > 32 && THREADS <= 256 && CNT <= 2;
 
 template <int CNT, int THREADS, bool ALIGNED, bool QUANTIZE, bool BF16>
 __global__ void __launch_bounds__(kTeamBlock<THREADS>, (kNormBlocksPerSm<CNT, THREADS, ALIGNED>)) residual_norm_kernel(const ResidualNormParams p) {
