@@ -406,6 +406,29 @@ def test_residual_norm(n, dtype):
         _near_quantized(q, scale, want, off_y)
 
 
+# many rows: a width for every number of threads and of 8-element units a thread, of rows that start on 16 bytes and of others
+MANY = [8 * u for u in (20, 40, 72, 104, 136, 168, 200, 264, 328, 400, 520, 648, 800, 1032, 1300, 1544, 2056, 2568, 3080)]
+MANY += [200 - 7, 505, 761, 1001, 1529, 2041, 2901, 4001, 6001, 8001, 12001, 16001, 24001]
+
+
+@pytest.mark.parametrize("n", MANY)
+def test_many_rows(n):
+    dtype = DTYPES[n // 8 % 2]
+    x = torch.randn(601, n, generator=_gen(n), device="cuda").to(dtype)
+    q, scale = kernels.quantize_rows(x)
+    want, ws = _quantized64(x.double())
+    assert torch.equal(q.double(), want)
+    assert bool(((scale.double() - ws.flatten()).abs() <= STEP32 * ws.flatten()).all())
+    x, o = _norm_operands(304, n, dtype, n, 4, (None, "rms", "layer")[n % 3], ("layer", "rms")[n % 2])
+    (total, off_t), (want, off_y) = _residual_norm64(x, o)
+    s, y = kernels.residual_norm(x, **o)
+    _close(s, total, off_t, dtype)
+    _close(y, want, off_y, dtype)
+    s8, q, scale = kernels.residual_norm(x, quantize=True, **o)
+    assert torch.equal(s8, s)
+    _near_quantized(q, scale, want, off_y)
+
+
 @pytest.mark.parametrize("leave_out", [("residual",), ("gate",), ("gamma", "beta"), ("post_gamma",), ("post_beta", "beta"),
                                        ("residual", "gate", "post_gamma", "post_beta", "gamma", "beta")])
 @pytest.mark.parametrize("n", [768, 1001, 2048])
