@@ -14,6 +14,7 @@ struct QuantizeParams {
   int8_t* q;
   float* scale;
   long long rows, x_pitch, q_pitch;
+  InnerRows inside;
   int n, activation;
 };
 
@@ -29,7 +30,7 @@ __global__ void __launch_bounds__(kTeamBlock<THREADS>) quantize_rows_kernel(cons
   const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.x_pitch;
   const uint16_t* lo = static_cast<const uint16_t*>(p.x);
   const uint16_t* hi = lo + (p.rows - 1) * p.x_pitch + (GATED ? 2 * p.n : p.n);
-  const bool inner = row > 0 && row < p.rows - 1;
+  const bool inner = row >= p.inside.begin && row < p.inside.end;
   const Team team(words, p.n, x);
   uint4 raw[CNT], up[GATED ? CNT : 1];
 #pragma unroll
@@ -129,7 +130,8 @@ B200AIT_EXPORT int b200ait_quantize_rows(void* q, float* scale, const void* x, i
     B200AIT_REQUIRE(multiple_of(x, 2) && multiple_of(scale, 4), "quantize_rows: a pointer is not aligned to its type");
     const bool lie_well = multiple_of(q, 8) && q_pitch % 8 == 0;
     const bool aligned = n % 8 == 0 && x_pitch % 8 == 0 && multiple_of(x, 16);
-    const QuantizeParams p{x, static_cast<int8_t*>(q), scale, rows, x_pitch, q_pitch, static_cast<int>(n), activation};
+    const QuantizeParams p{x, static_cast<int8_t*>(q), scale, rows, x_pitch, q_pitch, inner_rows(rows, x_pitch),
+                           static_cast<int>(n), activation};
     const bool bf16 = dtype == kDTypeBFloat16;
     if (gated && bf16)
       quantize_dispatch<true, true>(p, lie_well, aligned, stream);

@@ -29,6 +29,7 @@ struct ResidualNormParams {
   void *sum, *y;
   float* scale;  // of y in 8 bits
   long long rows, y_pitch;
+  InnerRows inside;  // of x and residual
   RowParts whole, gate_part, gamma_part, beta_part;  // whole: one vector for all rows
   int n, post, norm;
   float residual_scale, eps;
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(kTeamBlock<THREADS>, (kNormBlocksPerSm<CNT, TH
   const long long at = row * p.n, all = p.rows * p.n;
   const Team team(words, p.n, static_cast<const uint16_t*>(p.x) + at);
   const float inv_n = 1.f / static_cast<float>(p.n);
-  const bool inner = row > 0 && row < p.rows - 1;
+  const bool inner = row >= p.inside.begin && row < p.inside.end;
   uint4 xr[CNT], rr[CNT];
   auto fetch = [&](const void* tensor, uint4 (&raw)[CNT]) {
     const uint16_t* t = static_cast<const uint16_t*>(tensor);
@@ -284,7 +285,8 @@ B200AIT_EXPORT int b200ait_residual_norm(void* sum, void* y, float* y_scale, con
     B200AIT_REQUIRE(rows < (1ll << 31) && n < (1ll << 30), "residual_norm: dimension exceeds int32");
     const bool quantize = y_scale != nullptr;
     B200AIT_REQUIRE(!quantize || y_pitch >= n, "residual_norm: a row pitch is shorter than the row");
-    ResidualNormParams p{x, residual, gate, post_gamma, post_beta, gamma, beta, sum, y, y_scale, rows, y_pitch, {}, {}, {}, {},
+    ResidualNormParams p{x, residual, gate, post_gamma, post_beta, gamma, beta, sum, y, y_scale, rows, y_pitch, inner_rows(rows, n),
+                         {}, {}, {}, {},
                          static_cast<int>(n), post_norm, norm, residual_scale, eps};
     p.whole.rows = static_cast<int>(rows);
     p.whole.mul = FastDiv(p.whole.rows).mul, p.whole.shr = FastDiv(p.whole.rows).shr;

@@ -96,8 +96,8 @@ struct RowTeam {
     return v;
   }
 
-  // Unit i of row r of `rows` whose memory starts at `lo` and ends at `hi`. What is not the row's holds anything (clear_rest): a unit
-  // that reaches over the row's ends takes its neighbours' elements along.
+  // Unit i of a row of an operand whose memory starts at `lo` and ends at `hi`. What is not the row's holds anything (clear_rest): a unit
+  // that reaches over the row's ends takes its neighbours' elements along, which are the operand's own for an `inner` row (inner_rows).
   __device__ __forceinline__ uint4 load(const uint16_t* row, bool inner, const uint16_t* lo, const uint16_t* hi, int i) const {
     if (!has(i)) return make_uint4(0, 0, 0, 0);
     const uint16_t* at = row - skew + unit(i) * 8;

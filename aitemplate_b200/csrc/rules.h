@@ -276,4 +276,15 @@ inline bool blocks_start_early(long long blocks, int threads, int sms, int fille
   return 2 * blocks <= sms || blocks * threads >= static_cast<long long>(filled_threads) * sms || (light && blocks <= 4ll * sms);
 }
 
+// Rows in registers (rowteam.cuh): a skewed row is read in the 16-byte pieces of memory that hold it, the first and last of which take up
+// to 7 elements of its neighbours along. In these rows [begin, end) of `rows` at a pitch of `pitch` elements that stays inside the
+// operand, whatever the skew; a row nearer to its ends than that has its end pieces read element by element.
+struct InnerRows {
+  long long begin, end;
+};
+inline InnerRows inner_rows(long long rows, long long pitch) {
+  const long long away = pitch >= 7 ? 1 : (7 + pitch - 1) / pitch;
+  return InnerRows{away, rows - away};
+}
+
 }  // namespace b200ait
