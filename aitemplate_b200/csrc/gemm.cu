@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(256) gemm_simt_i8_kernel(const int8_t* a, cons
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = row0 + ty + i * 8;
-    if (row < p.M) epilogue_scalar_store_i8<BF16>(p, __int2float_rn(acc[i]) * cs, p.row_scale[row], row, col);
+    if (row < p.M) epilogue_scalar_store_i8<BF16>(p, scale_column_i8(acc[i], cs), p.row_scale[row], row, col);
   }
 }
 

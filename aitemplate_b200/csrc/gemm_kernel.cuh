@@ -252,11 +252,14 @@ __device__ __forceinline__ void epilogue_scalar_store(const GemmParams& p, float
   if (p.bias) v += Elem16<BF16>::to_float(static_cast<const typename Elem16<BF16>::T*>(p.bias)[col]);
   epilogue_scalar_rest<BF16>(p, v, b, row, col);
 }
-// The same on a sum of 8-bit products times its column's scale, with its row's scale, rounded as the tile kernels round.
+// A sum of 8-bit products times its column's scale, and that times its row's plus the bias: as the tile kernels round, and as they do without
+// flushing (rows of bf16 values under 2^-119 have scales that are no normal numbers, but results that are).
+__device__ __forceinline__ float scale_column_i8(int sum, float cs) { return mul_exact(__int2float_rn(sum), cs); }
+__device__ __forceinline__ float scale_row_i8(float scaled, float rs, float bias) { return fma_exact(scaled, rs, bias); }
+// The fused epilogue on a sum times its column's scale.
 template <bool BF16>
 __device__ __forceinline__ void epilogue_scalar_store_i8(const GemmParams& p, float scaled, float rs, int row, int col) {
-  const float v = p.bias ? __fmaf_rn(scaled, rs, Elem16<BF16>::to_float(static_cast<const typename Elem16<BF16>::T*>(p.bias)[col]))
-                         : scaled * rs;
+  const float v = scale_row_i8(scaled, rs, p.bias ? Elem16<BF16>::to_float(static_cast<const typename Elem16<BF16>::T*>(p.bias)[col]) : 0.f);
   epilogue_scalar_rest<BF16, true>(p, v, 0, row, col);
 }
 

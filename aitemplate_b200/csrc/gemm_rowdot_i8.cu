@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kRowDotI8Threads, 1) gemm_rowdot_i8_kernel(con
     }
     const int i = lane / (32 / kValues), n = at_n + (i / MR) * kWarps, m = i % MR;
     if (lane % (32 / kValues) == 0 && n < n_end && m < p.M)
-      epilogue_scalar_store_i8<BF16>(p, __int2float_rn(val[0]) * p.col_scale[n], X_TYPE == 0 ? p.row_scale[m] : scales[m], m, n);
+      epilogue_scalar_store_i8<BF16>(p, scale_column_i8(val[0], p.col_scale[n]), X_TYPE == 0 ? p.row_scale[m] : scales[m], m, n);
   };
   while (n0 < n_end) {
     step(wa, wb);

@@ -246,6 +246,7 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_const
       // this thread's column of the slab while it adds up sums, and the factor of a row while the tile goes out
       const float col_scale = I8 && slab * 128 + row < p.N ? p.col_scale[slab * 128 + row] : 0.f;
       auto row_factor = [&](int r) { return I8 ? p.row_scale[r] : p.alpha; };
+      auto scaled = [](float v, float factor, float bias) { return I8 ? scale_row_i8(v, factor, bias) : v * factor + bias; };
       ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, kDevWaitAccFullTimeout);
       if (!ok) break;
       tc_fence_after();
@@ -316,7 +317,7 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_const
                 }
               }
 #pragma unroll
-              for (int j = 0; j < kChunk; ++j) tile[(c * kChunk + j) * 128 + row] = __int2float_rn(sum[j]) * col_scale;
+              for (int j = 0; j < kChunk; ++j) tile[(c * kChunk + j) * 128 + row] = scale_column_i8(sum[j], col_scale);
             } else {
               float sum[kChunk];
 #pragma unroll
@@ -369,7 +370,7 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_const
             const float4 a0 = *reinterpret_cast<const float4*>(src), a1 = *reinterpret_cast<const float4*>(src + 4);
             float w[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = w[e] * factor + bias_v[e];
+            for (int e = 0; e < 8; ++e) w[e] = scaled(w[e], factor, bias_v[e]);
             apply_unary_vec_of<I8>(u1, w);
             *reinterpret_cast<float4*>(src) = make_float4(w[0], w[1], w[2], w[3]);
             *reinterpret_cast<float4*>(src + 4) = make_float4(w[4], w[5], w[6], w[7]);
@@ -400,7 +401,7 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_const
               if (j + 8 * t < my_rows) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                  const float y = pre ? o[t][e] : o[t][e] * factor[t] + bias_v[e];
+                  const float y = pre ? o[t][e] : scaled(o[t][e], factor[t], bias_v[e]);
                   o[t][e] = relu ? fmaxf(y, 0.f) : y;  // identity keeps a NaN a NaN
                 }
                 if (add_d0) {
@@ -438,7 +439,7 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_const
             if (!pre) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
-                const float y = o[i] * factor[i >> 3] + bias_v[i & 7];
+                const float y = scaled(o[i], factor[i >> 3], bias_v[i & 7]);
                 o[i] = u1 == kUnaryRelu ? fmaxf(y, 0.f) : y;
               }
             }

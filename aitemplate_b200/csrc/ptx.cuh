@@ -452,6 +452,17 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// One value of the same: like the pairs, and unlike the compiler's arithmetic here, these do not flush values under 2^-126 to zero.
+__device__ __forceinline__ float mul_exact(float a, float b) {
+  float d;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float fma_exact(float a, float b, float c) {
+  float d;
+  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // Kernels launched by launch_early (common.h) may be resident before the kernel ahead of them on the stream has finished:
 // everything that reads or writes global memory comes after grid_wait, which every thread of every CTA calls (a CTA that left

@@ -206,11 +206,6 @@ struct RowScale {
   float prescale, amax, inv, back;  // amax after prescaling, 127 / amax, 1 / amax
   bool flat;                  // all q are 0: a row of zeros (scale 0), or one with an infinity or NaN in it (scale NaN)
 };
-__device__ __forceinline__ float mul_exact(float a, float b) {  // without flushing small values to zero
-  float r;
-  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ RowScale row_scale_of(uint32_t amax_bits) {
   RowScale s;
   const float amax = __uint_as_float(amax_bits);
