@@ -198,6 +198,7 @@ void run_rowdot_i8(const void* x, int x_type, const void* w, const GemmParams& p
 #undef B200AIT_KVS
 #undef B200AIT_ONE
   }
+  throw Error("no kernel for as many rows of 8-bit integers");
 }
 
 }  // namespace b200ait

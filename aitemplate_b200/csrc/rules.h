@@ -239,17 +239,27 @@ inline bool gemm_may_split(long long m, long long n, long long k) {
   return !(m >= 5 && n >= 128) && !gemm_rowdot_long(m, n, k);
 }
 
-// GEMM of 8-bit integers, a few rows of X: on the CUDA cores (gemm_rowdot_i8.cu) or, from 128 columns and K = 256 on, by the weight-streaming
-// kernel, whose time does not grow with the rows. us, CUDA cores with 1 / 2 / 4 rows and the other: 4096 x 4096 5.5 / 6.4 / 7.7, 5.9;
-// 1024 x 1024 2.1 / 2.7 / 4.0, 3.2; 2048 x 2048 3.0 / 3.5 / 4.4, 4.2; 1024 x 4096 2.9 / 3.4 / 4.3, 4.5; 8192 x 8192 12.8 / 13.4 / 18.2, 12.8;
-// 14336 x 4096 12.0 / 13.2 / 17.7, 11.8; 4096 x 512 2.5 / 3.8 / 6.8, 3.1; 16384 x 1024 5.3 / 5.7 / 9.0, 7.1. With X in 16 bits
-// the other one needs a launch ahead of it to quantise them, which the CUDA cores do on the way: 2 rows 3.9 and 5.7 (2048 x 2048), 6.7 and
-// 7.6 (4096 x 4096), 4 rows 6.1 and 5.7, 9.7 and 7.6, and 3 us less on the host, which sets the pace of calls of this size.
+// GEMM of 8-bit integers, a few rows of X: on the CUDA cores (gemm_rowdot_i8.cu), or by the kernels that take more rows and whose time does
+// not grow with them: weight streaming from 128 columns and K = 511 on (its planner counts 8-bit operands as 16-bit ones of half the depth),
+// tiles below. us in a graph, CUDA cores / the others, W in L2, and in brackets from HBM, other weights at every call:
+//   1 row    1024 x 256 2.1 / 2.6 (2.2 / 3.1), 4096 x 1024 2.3 / 3.4 (2.9 / 4.0), 4096 x 4096 3.7 / 5.1 (5.6 / 5.8), 8192 x 8192 7.5 / 8.5 (12.7 / 12.7)
+//   2 rows   K > 512: 1024 x 640 2.6 / 3.1 (2.8 / 3.5), 8192 x 1024 2.9 / 3.5 (3.9 / 4.5), 16384 x 1024 4.2 / 6.5 (5.6 / 7.1), 4096 x 2048 3.1 / 4.1 (4.2 / 4.7),
+//            2048 x 4096 3.2 / 4.1 (4.3 / 4.8); beyond what the rule sends, 32768 x 1024 6.7 / 6.7 (8.4 / 8.8), 8192 x 2048 4.3 / 4.5 (6.3 / 5.7),
+//            4096 x 4096 4.5 / 5.1 (6.4 / 5.9), 8192 x 8192 9.7 / 8.6 (13.4 / 12.7).
+//            Up to 512 a warp's step is eight columns of one vector a lane, and their sums over the lanes set the pace: 4096 x 64 3.7 / 2.7 (3.9 / 3.1), 4096 x 256
+//            3.7 / 2.9 (3.9 / 3.2), 1024 x 320 3.3 / 2.7, 4096 x 480 3.8 / 3.8 (4.0 / 4.0), 16384 x 512 3.9 / 4.6 (5.0 / 5.1), 8192 x 384 3.7 / 4.5 (4.2 / 5.1).
+//            Under 128 columns a tile walks K alone: 8 x 4096 2.5 / 6.5, 127 x 2048 2.4 / 4.6, but 64 x 64 3.2 / 2.2
+// With X in 16 bits the others need a launch ahead of them to quantise it, which the CUDA cores do on the way, and that saves 3 us on the host, which
+// sets the pace of single calls of this size. In a graph:
+//   2 rows   4096 x 128 4.5 / 3.7 (4.7 / 4.1), 4096 x 1024 3.6 / 4.6 (4.2 / 5.2), 4096 x 4096 5.6 / 6.5 (7.4 / 7.4), 8192 x 8192 11.7 / 10.1 (15.2 / 14.8)
+//   4 rows   1024 x 768 5.4 / 4.6 (5.6 / 5.0), 2048 x 2048 5.4 / 5.1 (6.0 / 5.5), 100 x 4096 5.5 / 8.0, but 4096 x 4096 8.3 / 6.5 (10.0 / 7.4), and up to K = 512
+//            4096 x 256 11.1 / 4.1 (11.2 / 4.3)
 inline bool gemm_i8_rowdot(long long m, long long n, long long k, bool x16) {
   constexpr long long kShared = 160 << 10;  // for the rows of X
   if (m < 1 || m > 4 || (m <= 2 ? m : 4) * ((k + 15) / 16 * 16) > kShared) return false;
-  if (m == 1 || (m == 2 && (x16 || n < 128 || k < 256))) return true;
-  return n * k <= (m == 2 ? 8ll << 20 : 4ll << 20) && (x16 || (m == 2 && k >= 1024));
+  if (m == 1 || (m == 2 && (x16 || n < 128))) return true;
+  if (k <= 512) return false;
+  return m == 2 ? n * k <= (k <= 1024 ? 16ll << 20 : 8ll << 20) : x16 && n * k <= 4ll << 20;
 }
 
 // May a tile kernel's CTAs become resident before the kernel ahead of it has ended (launch_early)? It saves 0.4 .. 0.8 us (3 .. 25 %
