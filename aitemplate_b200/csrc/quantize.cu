@@ -123,7 +123,8 @@ B200AIT_EXPORT int b200ait_quantize_rows(void* q, float* scale, const void* x, i
     B200AIT_REQUIRE(dtype == kDTypeHalf || dtype == kDTypeBFloat16, "quantize_rows: dtype must be float16 or bfloat16");
     B200AIT_REQUIRE(rows >= 0 && n >= 0, "quantize_rows: negative dimension");
     B200AIT_REQUIRE(activation >= kUnaryIdentity && activation <= kUnaryHardswish, "quantize_rows: unknown activation");
-    if (rows == 0 || n == 0) return;
+    if (rows == 0) return;
+    B200AIT_REQUIRE(n != 0, "quantize_rows: the rows have no columns");  // (and so no largest value to scale by)
     B200AIT_REQUIRE(q && scale && x, "quantize_rows: null pointer with non-zero size");
     B200AIT_REQUIRE(rows < (1ll << 31) && n < (1ll << 30), "quantize_rows: dimension exceeds int32");
     B200AIT_REQUIRE(x_pitch >= (gated ? 2 * n : n) && q_pitch >= n, "quantize_rows: a row pitch is shorter than the row");

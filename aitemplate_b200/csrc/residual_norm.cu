@@ -280,7 +280,9 @@ B200AIT_EXPORT int b200ait_residual_norm(void* sum, void* y, float* y_scale, con
     B200AIT_REQUIRE(norm == kNormLayer || norm == kNormRms, "residual_norm: the norm is layer (1) or rms (2)");
     B200AIT_REQUIRE(post_norm >= kNormNone && post_norm <= kNormRms, "residual_norm: the norm after the block is none (0), layer (1) or rms (2)");
     B200AIT_REQUIRE(post_norm != kNormNone || (!post_gamma && !post_beta), "residual_norm: post_gamma and post_beta need a norm after the block");
-    if (rows == 0 || n == 0) return;
+    if (rows == 0) return;
+    B200AIT_REQUIRE(n != 0 || !y_scale, "residual_norm: the rows have no columns");  // (and so no largest value to scale by)
+    if (n == 0) return;
     B200AIT_REQUIRE(x && y, "residual_norm: null pointer with non-zero size");
     B200AIT_REQUIRE(rows < (1ll << 31) && n < (1ll << 30), "residual_norm: dimension exceeds int32");
     const bool quantize = y_scale != nullptr;
