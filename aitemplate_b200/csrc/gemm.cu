@@ -743,7 +743,10 @@ void gemm_run(const GemmArgs& g_in) {
   // few rows of X, or few output tiles: the weight-streaming kernel where its planner takes the problem
   const bool streams = tma_ok && g.batch == 1 && !g.b_mn && g.num_out == 1 && g.tile_n == 0 && g.split_k == 0;
   // (row-major B: its boxes are not rows of K, and the figures of rules.h do not hold)
-  // (8-bit operands count as 16-bit ones of half the length: the estimates are about boxes of 128 bytes and their MMAs)
+  // (8-bit operands count as 16-bit ones of half the length: the estimates are about boxes of 128 bytes and their MMAs. Over 50 problems of 6 .. 8192
+  // rows, 64 .. 8192 columns and depths the kernel so chosen takes 2.0 % longer on average than the best of it and the four widths, 22 % at
+  // worst: 120 x 7296 x 768 5.8 us, with 128-wide tiles 4.8. Where N is no multiple of 8 the estimates are those of the 16-bit loop, which
+  // takes longer than the 8-bit one; the 16 such problems among them are 2.6 % behind on average, 15 % at worst, 46 x 2043 x 128 6.0 us, 64-wide 5.2)
   const long long lda = g.i8 ? g.lda / 2 : g.lda, ldb = g.i8 ? g.ldb / 2 : g.ldb, k16 = g.i8 ? (g.k + 1) / 2 : g.k;
   const long long pitch = g.b_mn ? kBK : gemm_copy_row_us(lda) > gemm_copy_row_us(ldb) ? lda : ldb;
   GemmProblem problem{g.batch, g.m, g.n, k16, 0, 0, pitch, g.b_mn || g.num_out > 1};

@@ -62,7 +62,8 @@ __global__ void __launch_bounds__(kTeamBlock<THREADS>) quantize_rows_kernel(cons
 }
 
 // Rows longer than the registers of a block hold (32768 elements), or results at an odd place: a block walks its row twice, the
-// second time out of L2.
+// second time out of L2. Bound by its loads of single elements: 1000 x 40000 takes 116 us, gated 2 x 40000 (swish) 109, where HBM would take 18 and
+// 31; 1000 x 32768, which fits, 25 and 39.
 template <bool BF16>
 __global__ void __launch_bounds__(kTeamMaxThreads) quantize_long_rows_kernel(const QuantizeParams p, const bool gated) {
   using E = Elem16<BF16>;

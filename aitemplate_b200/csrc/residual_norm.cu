@@ -173,8 +173,9 @@ __global__ void __launch_bounds__(kTeamBlock<THREADS>, (kNormBlocksPerSm<CNT, TH
   }
 }
 
-// Rows longer than the registers of a block hold, or operands that do not lie alike: a block walks its row once for each statistic and once to write, after the first
-// time out of L2, and works the sum out anew each time.
+// Rows longer than the registers of a block hold, or operands that do not lie alike: a block walks its row once for each statistic and once to write,
+// after the first time out of L2, and works the sum out anew each time. Bound by its loads of single elements: 1000 x 40000 with a residual takes 204 us
+// (rms), 239 to 8 bits, 350 with both norms and a gate, where HBM would take 49, 43 and 49; 1000 x 32768, which fits, 47.
 template <bool QUANTIZE, bool BF16>
 __global__ void __launch_bounds__(kTeamMaxThreads) residual_norm_long_rows_kernel(const ResidualNormParams p) {
   using E = Elem16<BF16>;

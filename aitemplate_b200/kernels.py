@@ -432,8 +432,9 @@ def quantize_rows(x: torch.Tensor, activation: str = "identity", gated: bool = F
     """(q, scale): the rows (last dim) of act(x) as int8 with an fp32 scale each, the left operand of gemm_rcr_i8.
     scale = max |v| / 127, q = round(127 v / max |v|), ties to even. With `gated` x holds the two halves of a gated
     feed-forward's first product, and v = act(x[..., :n]) * x[..., n:]. A row of v that is all zeros gets scale 0; one with an
-    infinity or a NaN in it gets scale NaN and zeros. Rows of x may lie apart. Where n is not a multiple of 16, q is a view of rows padded
-    to 16 bytes, so that the product can read them with the tensor cores."""
+    infinity or a NaN in it gets scale NaN and zeros (relu makes 0 of a NaN, as in the GEMMs). Rows of x may lie apart.
+    Where n is not a multiple of 16, q is a view of rows padded to 16 bytes, so that the product can read them with the tensor
+    cores."""
     y = (_calls or _native()).quantize_rows(x, UNARY.get(activation), gated)
     if y is not None:
         return y

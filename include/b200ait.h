@@ -237,9 +237,9 @@ int b200ait_layernorm(void* out, const void* in, const void* gamma, const void* 
 
 /* Rows of 16-bit values to signed 8-bit ones with a scale each: q = round(127 v / max |v|) to the nearest, ties to even, and scale =
  * max |v| / 127, with v = act(x[:, :n]), or with `gated` act(x[:, :n]) * x[:, n:2n]. A row of v that is all zeros has scale 0 and q 0, one
- * with an infinity or a NaN in it scale NaN and q 0 (the relu of a NaN is 0, as in the GEMMs). Row pitches in elements; bytes of q between n and its pitch are left alone. Rows without columns (n = 0)
- * have no scale and are refused. `activation`:
- * one of B200AIT_UNARY_*. No counterpart in the reference. */
+ * with an infinity or a NaN in it scale NaN and q 0 (the relu of a NaN is 0, as in the GEMMs). Row pitches in elements; bytes of q
+ * between n and its pitch are left alone. Rows without columns (n = 0) have no scale and are refused. `activation`: one of
+ * B200AIT_UNARY_*. No counterpart in the reference. */
 int b200ait_quantize_rows(void* q, float* scale, const void* x, int64_t rows, int64_t n, int64_t x_pitch, int64_t q_pitch,
                           int activation, int gated, int dtype, b200ait_stream_t stream);
 
