@@ -914,6 +914,9 @@ B200AIT_EXPORT int b200ait_gemm_rcr(const void* a, const void* b, const void* bi
 static void check_i8(const GemmArgs& g, const float* b_scale) {
   B200AIT_REQUIRE(g.dtype == kDTypeHalf || g.dtype == kDTypeBFloat16, "gemm: dtype must be float16 or bfloat16");
   B200AIT_REQUIRE(g.m >= 0 && g.n >= 0 && g.k >= 0, "gemm: negative dimension");
+  // (the kernels count past the last row and column, up to two 256-row tiles or a step of eight columns for 16 warps and as much ahead)
+  constexpr long long kMost = (1ll << 31) - 1024;
+  B200AIT_REQUIRE(g.m <= kMost && g.n <= kMost, "gemm: dimension exceeds int32");
   // sums of K products of at most 2^14 each stay below 2^31
   B200AIT_REQUIRE(g.k < (1 << 17), "gemm: 8-bit operands take up to 131071 columns");
   if (g.m == 0 || g.n == 0) return;
