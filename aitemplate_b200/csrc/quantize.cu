@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kTeamMaxThreads) quantize_long_rows_kernel(con
   const T* x = static_cast<const T*>(p.x) + row * p.x_pitch;
   auto value = [&](int i) {
     const float v = apply_unary_of<true>(p.activation, E::to_float(x[i]));
-    return gated ? v * E::to_float(x[p.n + i]) : v;
+    return gated ? mul_exact(v, E::to_float(x[p.n + i])) : v;  // (as the pairs of the other kernel: small products are not flushed)
   };
   uint32_t most = 0;
   for (int i = team.tid; i < p.n; i += kTeamMaxThreads) {
